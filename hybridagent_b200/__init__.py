@@ -3,6 +3,7 @@
 The compute path is ``lib/libhybridagent_b200.so`` (hand-written CUDA + NCCL behind the C ABI
 of ``include/hybridagent_b200.h``); this package is its Python host side.
 """
+from .muon import ZeroOneMuon, orthogonalize
 from .optimizer import ZeroOneAdamW
 
-__all__ = ["ZeroOneAdamW"]
+__all__ = ["ZeroOneAdamW", "ZeroOneMuon", "orthogonalize"]

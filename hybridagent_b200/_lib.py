@@ -40,6 +40,19 @@ class Peers(ctypes.Structure):
     _fields_ = [("n", ctypes.c_int32), ("reserved", ctypes.c_int32), ("delta", ctypes.c_int64 * 15)]
 
 
+HA_NS_MAX_STEPS = 16
+
+
+class NsParams(ctypes.Structure):
+    _fields_ = [("steps", ctypes.c_int32), ("reserved", ctypes.c_int32), ("eps", ctypes.c_double),
+                ("coef", ctypes.c_float * (3 * HA_NS_MAX_STEPS))]
+
+
+class MuonScalars(ctypes.Structure):
+    _fields_ = [("mu", ctypes.c_float), ("one_minus_mu", ctypes.c_float), ("nesterov", ctypes.c_int32),
+                ("use_decay", ctypes.c_int32), ("clip", ctypes.c_int32), ("clip_mult", ctypes.c_float)]
+
+
 class HAError(RuntimeError):
     """A non-zero status from the C ABI, with the library's message."""
 
@@ -80,6 +93,11 @@ SIGNATURES: dict[str, tuple[list, object]] = {
                              ctypes.POINTER(Peers), _vp], ctypes.c_int),
     "ha_adamw_step_delta": ([_vp, _vp, _i64, _i64, ctypes.c_int, ctypes.POINTER(AdamwScalars), _vp, _vp, _vp],
                             ctypes.c_int),
+    "ha_orthogonalize_workspace": ([_i64, _i64, _i64, ctypes.POINTER(_sz)], ctypes.c_int),
+    "ha_orthogonalize": ([_vp, ctypes.c_int, _vp, _i64, _i64, _i64, ctypes.POINTER(NsParams), _vp, _sz, _vp],
+                         ctypes.c_int),
+    "ha_muon_step": ([_vp, _i64, _i64, _i64, ctypes.c_int, ctypes.POINTER(MuonScalars), ctypes.POINTER(NsParams),
+                      ctypes.c_int, ctypes.POINTER(Peers), _vp, _vp, _vp, _sz, _vp], ctypes.c_int),
     "ha_comm_unique_id": ([_vp], ctypes.c_int),
     "ha_comm_init": ([_vp, _i32, _i32, ctypes.POINTER(ctypes.c_void_p)], ctypes.c_int),
     "ha_comm_destroy": ([_vp], ctypes.c_int),

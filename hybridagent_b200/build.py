@@ -26,7 +26,7 @@ LIB_PATH = os.path.join(LIB_DIR, "libhybridagent_b200.so")
 CUDA_HOME = os.environ.get("CUDA_HOME", "/usr/local/cuda")
 NVCC = os.path.join(CUDA_HOME, "bin", "nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
-CU_SOURCES = ["adamw.cu", "gradnorm.cu", "gather.cu", "p2p.cu"]
+CU_SOURCES = ["adamw.cu", "gradnorm.cu", "gather.cu", "p2p.cu", "newton_schulz.cu", "muon.cu"]
 CPP_SOURCES = ["host.cpp", "comm.cpp"]
 
 
@@ -40,6 +40,7 @@ def _nccl_include() -> str:
 def _sources() -> list[str]:
     files = [os.path.join(CSRC, f) for f in CU_SOURCES + CPP_SOURCES]
     files += [os.path.join(CSRC, "ha_common.cuh"), os.path.join(CSRC, "ha_nvtx.h"),
+              *(os.path.join(CSRC, f) for f in ("ha_param.cuh", "umma.cuh", "newton_schulz.cuh")),
               os.path.join(INCLUDE, "hybridagent_b200.h"), __file__]
     return files
 

@@ -13,6 +13,7 @@
 // 256-byte (16-bit) segment.  Tensors whose pointers are not 16-byte aligned (possible
 // for caller-owned gradients) take a scalar path with identical arithmetic.
 #include "ha_common.cuh"
+#include "ha_param.cuh"
 
 namespace ha {
 namespace {
@@ -48,48 +49,6 @@ __device__ __forceinline__ void adamw_elem(const Scalars& s, float decay, float 
 template <int DT>
 __device__ __forceinline__ float grad_in(const Scalars& s, float g) {
   return s.clip ? clip_round<DT>(g, s.clip_mult) : g;
-}
-
-struct Peers {
-  int n;
-  int64_t delta[HA_MAX_PEERS];
-};
-
-// Four values rounded to a 16-bit DT, packed as one 8-byte word.
-template <int DT>
-__device__ __forceinline__ uint2 pack4(float4 x) {
-  return make_uint2(uint32_t(Elem<DT>::narrow(x.x)) | (uint32_t(Elem<DT>::narrow(x.y)) << 16),
-                    uint32_t(Elem<DT>::narrow(x.z)) | (uint32_t(Elem<DT>::narrow(x.w)) << 16));
-}
-
-// The same 8 bytes at `local` + e in every peer's copy of the packed parameter buffer.
-__device__ __forceinline__ void push_raw4(const Peers& p, uint64_t local, int64_t e, uint2 w) {
-#pragma unroll
-  for (int q = 0; q < HA_MAX_PEERS; ++q) {  // constant indices keep delta[] in the parameter bank
-    if (q >= p.n) break;
-    __stcs(reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(local + p.delta[q]) + e), w);
-  }
-}
-
-__device__ __forceinline__ void push_f32x4(const Peers& p, uint64_t local, int64_t e, float4 x) {
-#pragma unroll
-  for (int q = 0; q < HA_MAX_PEERS; ++q) {
-    if (q >= p.n) break;
-    store4_f32(reinterpret_cast<float*>(local + p.delta[q]), e, x);
-  }
-}
-
-template <int DT>
-__device__ __forceinline__ void push1(const Peers& p, uint64_t local, int64_t k, float x) {
-#pragma unroll
-  for (int q = 0; q < HA_MAX_PEERS; ++q) {
-    if (q >= p.n) break;
-    if constexpr (DT == HA_F32) {
-      reinterpret_cast<float*>(local + p.delta[q])[k] = x;
-    } else {
-      reinterpret_cast<uint16_t*>(local + p.delta[q])[k] = Elem<DT>::narrow(x);
-    }
-  }
 }
 
 // DT is the gradient and parameter dtype.  For HA_F32 the master is the parameter

@@ -1,0 +1,667 @@
+// Muon: momentum, orthogonalised update and weight update of matrices (sm_100a).
+//
+// For a matrix W with gradient G (K. Jordan's Muon; the momentum form of torch.optim.Muon):
+//     M <- mu M + (1 - mu) G,   U = (1 - mu) G + mu M  (look-ahead)  or  U = M
+//     O = five Newton-Schulz steps of U / max(|U|_F, eps)                (newton_schulz.cu)
+//     W <- W (1 - lr wd) - lr s O
+//
+// The element-wise kernels here are bound by HBM: per element of bf16 parameters the momentum kernel
+// moves 10 bytes (G, M read, M written) and sums U's squares; the load kernel reads G and M again
+// (6 bytes; U itself is never stored, which would round it before its norm is known) and writes
+// the two fp16 planes of U / |U|; the weight kernel reads O and the master and writes the master and
+// the changed sectors of the copy.  A launch takes its tensors' descriptors as kernel parameters
+// (kSlice of them), so a step uploads no table and can be captured into a graph.
+//
+// Sums: squares are taken and added in fp64 (gradients of 1e-30 or 1e25 keep their norm), each CTA
+// writes its own partial, and every reader adds a matrix's partials in the same order, so results
+// do not depend on scheduling.
+#include <cmath>
+
+#include "ha_common.cuh"
+#include "ha_param.cuh"
+#include "newton_schulz.cuh"
+
+namespace ha {
+namespace {
+
+constexpr int kSlice = 48;               // tensors of one launch: 48 x 64 bytes of kernel parameters
+constexpr int64_t kMinChunk = 8192;      // elements of one partial sum at least
+constexpr int64_t kMaxPartials = 512;    // partial sums of one matrix at most
+constexpr int kLoadChunk = kThreads * 8 * 4;  // padded elements of a CTA of the load and store kernels
+constexpr int64_t kApplyChunk = 16384;
+constexpr int kGroups = 4;               // 4-element groups per thread and pass of the weight kernel
+constexpr size_t kHeader = 256;          // the workspace's error word
+
+struct Slice {
+  ha_tensor t[kSlice];
+};
+
+struct MuonConst {
+  float mu, a_mu;  // mu and 1 - mu
+  int nesterov, use_decay, clip;
+  float clip_mult;
+};
+
+int64_t chunk_for(int64_t numel) {
+  const int64_t c = (numel + kMaxPartials - 1) / kMaxPartials;
+  return (c + kMinChunk - 1) / kMinChunk * kMinChunk;
+}
+
+__device__ __forceinline__ double block_sum_all(double x, double* smem) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (lane == 0) smem[warp] = x;
+  __syncthreads();
+  x = 0.0;
+#pragma unroll
+  for (int w = 0; w < kThreads / 32; ++w) x += smem[w];
+  return x;  // in every thread
+}
+
+// Eight consecutive elements of a DT array (a 16-byte aligned address) as fp32.
+template <int DT>
+__device__ __forceinline__ void load8(const typename Elem<DT>::raw* p, float (&x)[8]) {
+  if constexpr (DT == HA_F32) {
+    const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+    x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+  } else {
+    const uint4 w = *reinterpret_cast<const uint4*>(p);
+    const uint32_t v[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[2 * i] = Elem<DT>::widen(uint16_t(v[i] & 0xffffu));
+      x[2 * i + 1] = Elem<DT>::widen(uint16_t(v[i] >> 16));
+    }
+  }
+}
+
+__device__ __forceinline__ void add_square(double& acc, float u) {
+  const double d = double(u);
+  acc = __fma_rn(d, d, acc);
+}
+
+// One element of the momentum and of the update direction.
+template <int DT>
+__device__ __forceinline__ float momentum_elem(const MuonConst& s, float g, float& m) {
+  if (s.clip) g = clip_round<DT>(g, s.clip_mult);
+  m = __fmaf_rn(s.a_mu, g, __fmul_rn(m, s.mu));
+  return s.nesterov ? __fmaf_rn(s.a_mu, g, __fmul_rn(m, s.mu)) : m;
+}
+// The direction from the momentum already updated.
+template <int DT>
+__device__ __forceinline__ float direction_elem(const MuonConst& s, float g, float m) {
+  if (!s.nesterov) return m;
+  if (s.clip) g = clip_round<DT>(g, s.clip_mult);
+  return __fmaf_rn(s.a_mu, g, __fmul_rn(m, s.mu));
+}
+
+// Square sums of plain matrices, `numel` elements each, one after another.  Grid: (partials, matrices).
+template <int DT>
+__global__ void __launch_bounds__(kThreads)
+    square_sum_kernel(const void* src, int64_t numel, int64_t chunk, double* partials, uint32_t* error) {
+  __shared__ double red[kThreads / 32];
+  using raw = typename Elem<DT>::raw;
+  if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0 && error != nullptr) *error = 0;
+  const raw* x = static_cast<const raw*>(src) + int64_t(blockIdx.y) * numel;
+  const int64_t begin = int64_t(blockIdx.x) * chunk, end = min(begin + chunk, numel);
+  double acc = 0.0;
+  int64_t e = begin + int64_t(threadIdx.x) * 8;
+  if ((reinterpret_cast<uintptr_t>(x) & 15) == 0) {
+    for (; e + 8 <= end; e += kThreads * 8) {
+      float v[8];
+      load8<DT>(x + e, v);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) add_square(acc, v[i]);
+    }
+    for (int64_t k = e; k < min(e + 8, end); ++k) add_square(acc, Elem<DT>::widen(x[k]));
+  } else {
+    for (int64_t k = begin + threadIdx.x; k < end; k += kThreads) add_square(acc, Elem<DT>::widen(x[k]));
+  }
+  acc = block_sum_all(acc, red);
+  if (threadIdx.x == 0) partials[int64_t(blockIdx.y) * gridDim.x + blockIdx.x] = acc;
+}
+
+// Momentum update and square sums of the direction.  Grid: (partials, tensors of the slice).
+template <int DT>
+__global__ void __launch_bounds__(kThreads)
+    momentum_kernel(const __grid_constant__ Slice s, MuonConst c, int64_t chunk, double* partials, uint32_t* error) {
+  __shared__ double red[kThreads / 32];
+  using raw = typename Elem<DT>::raw;
+  if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0 && error != nullptr) *error = 0;
+  const ha_tensor& t = s.t[blockIdx.y];
+  const raw* grad = reinterpret_cast<const raw*>(t.grad);
+  float* mom = reinterpret_cast<float*>(t.exp_avg);
+  const int64_t begin = int64_t(blockIdx.x) * chunk, end = min(begin + chunk, t.numel);
+  double acc = 0.0;
+  auto one = [&](int64_t k) {
+    float m = mom[k];
+    add_square(acc, momentum_elem<DT>(c, Elem<DT>::widen(grad[k]), m));
+    mom[k] = m;
+  };
+  if (((t.grad | t.exp_avg) & 15) == 0) {
+    int64_t e = begin + int64_t(threadIdx.x) * 8;
+    for (; e + 8 <= end; e += kThreads * 8) {
+      float g[8], m[8];
+      load8<DT>(grad + e, g);
+      load8<HA_F32>(mom + e, m);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) add_square(acc, momentum_elem<DT>(c, g[i], m[i]));
+      reinterpret_cast<float4*>(mom + e)[0] = make_float4(m[0], m[1], m[2], m[3]);
+      reinterpret_cast<float4*>(mom + e)[1] = make_float4(m[4], m[5], m[6], m[7]);
+    }
+    for (int64_t k = e; k < min(e + 8, end); ++k) one(k);
+  } else {
+    for (int64_t k = begin + threadIdx.x; k < end; k += kThreads) one(k);
+  }
+  acc = block_sum_all(acc, red);
+  if (threadIdx.x == 0) partials[int64_t(blockIdx.y) * gridDim.x + blockIdx.x] = acc;
+}
+
+struct Shape {
+  int64_t rows, cols, ld, plane;
+};
+
+// What the load kernel reads: element k of matrix `y` of the launch.
+template <int DT>
+struct PlainSource {
+  const typename Elem<DT>::raw* x;
+  int64_t numel;
+  struct View {
+    const typename Elem<DT>::raw* x;
+    __device__ bool aligned() const { return (reinterpret_cast<uintptr_t>(x) & 15) == 0; }
+    __device__ float one(int64_t k) const { return Elem<DT>::widen(x[k]); }
+    __device__ void eight(int64_t k, float (&v)[8]) const { load8<DT>(x + k, v); }
+  };
+  __device__ View view(int y) const { return View{x + y * numel}; }
+};
+template <int DT>
+struct MuonSource {
+  Slice s;
+  MuonConst c;
+  struct View {
+    const typename Elem<DT>::raw* g;
+    const float* m;
+    MuonConst c;
+    __device__ bool aligned() const {
+      return ((reinterpret_cast<uintptr_t>(g) | reinterpret_cast<uintptr_t>(m)) & 15) == 0;
+    }
+    __device__ float one(int64_t k) const { return direction_elem<DT>(c, Elem<DT>::widen(g[k]), m[k]); }
+    __device__ void eight(int64_t k, float (&v)[8]) const {
+      float a[8];
+      load8<DT>(g + k, a);
+      load8<HA_F32>(m + k, v);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = direction_elem<DT>(c, a[i], v[i]);
+    }
+  };
+  __device__ View view(int y) const {
+    return View{reinterpret_cast<const typename Elem<DT>::raw*>(s.t[y].grad),
+                reinterpret_cast<const float*>(s.t[y].exp_avg), c};
+  }
+};
+
+// X0 = U / max(|U|_F, eps) into the high and low planes of matrix first + blockIdx.y (row padding
+// left alone).  Grid: (chunks of the padded matrix, matrices).
+template <class Source>
+__global__ void __launch_bounds__(kThreads) load_kernel(const __grid_constant__ Source src, Shape sh, int n_partials,
+                                                        const double* partials, double eps, int first, __half* hi,
+                                                        __half* lo) {
+  __shared__ double red[kThreads / 32];
+  const double* part = partials + int64_t(blockIdx.y) * n_partials;
+  double sum = 0.0;
+  for (int i = threadIdx.x; i < n_partials; i += kThreads) sum += part[i];
+  const double norm = sqrt(block_sum_all(sum, red));
+  const float scale = float(double(kScaleX) / (norm < eps ? eps : norm));  // a NaN norm stays one
+  const typename Source::View v = src.view(blockIdx.y);
+  hi += (first + int64_t(blockIdx.y)) * sh.plane;
+  lo += (first + int64_t(blockIdx.y)) * sh.plane;
+  const bool vec = v.aligned() && (sh.cols & 7) == 0;
+  const uint32_t per_row = uint32_t(sh.ld >> 3);
+  const int64_t total = sh.rows * per_row;
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    const int64_t k = int64_t(blockIdx.x) * (kThreads * 4) + u * kThreads + threadIdx.x;
+    if (k >= total) break;
+    const uint32_t r = uint32_t(k) / per_row, c = (uint32_t(k) - r * per_row) * 8;
+    const int64_t e = int64_t(r) * sh.cols + c;
+    float x[8];
+    if (vec) {
+      v.eight(e, x);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = c + i < sh.cols ? v.one(e + i) : 0.0f;
+    }
+    uint32_t h[4], l[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float a = __fmul_rn(x[2 * i], scale), b = __fmul_rn(x[2 * i + 1], scale);
+      const __half2 p = __floats2half2_rn(a, b);
+      const float2 f = __half22float2(p);
+      const __half2 q = __floats2half2_rn((a - f.x) * kScaleLo, (b - f.y) * kScaleLo);
+      h[i] = *reinterpret_cast<const uint32_t*>(&p);
+      l[i] = *reinterpret_cast<const uint32_t*>(&q);
+    }
+    const int64_t at = int64_t(r) * sh.ld + c;
+    *reinterpret_cast<uint4*>(hi + at) = make_uint4(h[0], h[1], h[2], h[3]);
+    *reinterpret_cast<uint4*>(lo + at) = make_uint4(l[0], l[1], l[2], l[3]);
+  }
+}
+
+// The orthogonalised matrices as bf16 (NaN if a wait of the products ran out).
+__global__ void __launch_bounds__(kThreads)
+    store_kernel(const __half* x, Shape sh, uint16_t* out, const uint32_t* error) {
+  const bool bad = *error != 0;
+  x += int64_t(blockIdx.y) * sh.plane;
+  out += int64_t(blockIdx.y) * sh.rows * sh.cols;
+  const bool vec = (sh.cols & 7) == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
+  const uint32_t per_row = uint32_t(sh.ld >> 3);
+  const int64_t total = sh.rows * per_row;
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    const int64_t k = int64_t(blockIdx.x) * (kThreads * 4) + u * kThreads + threadIdx.x;
+    if (k >= total) break;
+    const uint32_t r = uint32_t(k) / per_row, c = (uint32_t(k) - r * per_row) * 8;
+    const uint4 w = *reinterpret_cast<const uint4*>(x + int64_t(r) * sh.ld + c);
+    const uint32_t v[4] = {w.x, w.y, w.z, w.w};
+    uint32_t b[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&v[i]));
+      b[i] = bad ? 0x7fff7fffu
+                 : uint32_t(Elem<HA_BF16>::narrow(f.x * (1.0f / kScaleX))) |
+                       (uint32_t(Elem<HA_BF16>::narrow(f.y * (1.0f / kScaleX))) << 16);
+    }
+    const int64_t e = int64_t(r) * sh.cols + c;
+    if (vec) {
+      *reinterpret_cast<uint4*>(out + e) = make_uint4(b[0], b[1], b[2], b[3]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (c + i < sh.cols) out[e + i] = uint16_t(b[i >> 1] >> (16 * (i & 1)));
+    }
+  }
+}
+
+// W <- W * decay + neg_lr * O, the copy of W in DT, and the peers' copies.  neg_lr holds the shape's
+// factor and the plane's scale.  The stores follow adamw_kernel's (changed sectors only with DELTA).
+template <int DT, bool PEERS, bool DELTA>
+__global__ void __launch_bounds__(kThreads)
+    apply_kernel(const __grid_constant__ Slice s, const __half* x, Shape sh, int first, int use_decay, Peers peers,
+                 unsigned long long* changed, const uint32_t* error, uint32_t* status) {
+  static_assert(!(DELTA && DT == HA_F32), "fp32 parameters are their own masters: always written");
+  __shared__ uint32_t stored_in_cta;
+  if (*error != 0) {  // a wait of the products ran out: the weights stay as they are
+    if (threadIdx.x == 0 && status != nullptr) atomicExch(status, 1u);
+    return;
+  }
+  const ha_tensor& t = s.t[blockIdx.y];
+  x += (first + int64_t(blockIdx.y)) * sh.plane;
+  float* master = reinterpret_cast<float*>(t.master);
+  void* param = reinterpret_cast<void*>(t.param);
+  const uint64_t pushed = DT == HA_F32 ? t.master : t.param;
+  const float decay = t.decay, lr = __fmul_rn(t.neg_lr, 1.0f / kScaleX);
+  const int64_t begin = int64_t(blockIdx.x) * kApplyChunk, end = min(begin + kApplyChunk, t.numel);
+  const bool vec = (t.master & 15) == 0 && (DT == HA_F32 || (t.param & 7) == 0);
+  const bool vec_x = (sh.cols & 3) == 0;
+  uint32_t stored = 0;
+  if (DELTA && threadIdx.x == 0) stored_in_cta = 0;
+  auto update = [&](float w, float o) {
+    if (use_decay) w = __fmul_rn(w, decay);
+    return __fmaf_rn(lr, o, w);
+  };
+  auto one = [&](int64_t k) {
+    const int64_t r = k / sh.cols, c = k - r * sh.cols;
+    const float before = master[k];
+    const float a = update(before, __half2float(x[r * sh.ld + c]));
+    master[k] = a;
+    if constexpr (DT != HA_F32) {
+      const uint16_t w = Elem<DT>::narrow(a);
+      if (!DELTA || w != Elem<DT>::narrow(before)) {
+        static_cast<uint16_t*>(param)[k] = w;
+        if constexpr (PEERS) push1<DT>(peers, pushed, k, a);
+        stored += DELTA;
+      }
+    } else if constexpr (PEERS) {
+      push1<DT>(peers, pushed, k, a);
+    }
+  };
+  if (vec) {
+    constexpr int64_t kPass = int64_t(kThreads) * kGroups * 4;
+    for (int64_t base = begin; base < end; base += kPass) {
+      float4 ms[kGroups], o[kGroups];
+      int64_t e[kGroups];
+#pragma unroll
+      for (int u = 0; u < kGroups; ++u) {
+        e[u] = base + 4 * (int64_t(threadIdx.x) + int64_t(u) * kThreads);
+        if (e[u] + 4 <= end) {
+          ms[u] = load4_f32(master, e[u]);
+          int64_t r = e[u] / sh.cols, c = e[u] - r * sh.cols;
+          if (vec_x) {
+            const uint2 w = *reinterpret_cast<const uint2*>(x + r * sh.ld + c);
+            const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&w.x));
+            const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&w.y));
+            o[u] = make_float4(a.x, a.y, b.x, b.y);
+          } else {
+            float v[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              v[i] = __half2float(x[r * sh.ld + c]);
+              if (++c == sh.cols) c = 0, ++r;
+            }
+            o[u] = make_float4(v[0], v[1], v[2], v[3]);
+          }
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < kGroups; ++u) {
+        const bool full = e[u] + 4 <= end;
+        uint2 w = make_uint2(0, 0);
+        bool moved = false;
+        if (full) {
+          uint2 before = make_uint2(0, 0);
+          if constexpr (DELTA) before = pack4<DT>(ms[u]);
+          ms[u].x = update(ms[u].x, o[u].x);
+          ms[u].y = update(ms[u].y, o[u].y);
+          ms[u].z = update(ms[u].z, o[u].z);
+          ms[u].w = update(ms[u].w, o[u].w);
+          store4_f32(master, e[u], ms[u]);
+          if constexpr (DT != HA_F32) {
+            w = pack4<DT>(ms[u]);
+            moved = w.x != before.x || w.y != before.y;
+          } else if constexpr (PEERS) {
+            push_f32x4(peers, pushed, e[u], ms[u]);
+          }
+        }
+        if constexpr (DT != HA_F32) {
+          bool store = full;
+          if constexpr (DELTA) {  // the four lanes of a 32-byte sector store together
+            uint32_t any = moved ? 1u : 0u;
+            any |= __shfl_xor_sync(0xffffffffu, any, 1);
+            any |= __shfl_xor_sync(0xffffffffu, any, 2);
+            store = full && any;
+          }
+          if (store) {
+            __stcs(reinterpret_cast<uint2*>(static_cast<uint16_t*>(param) + e[u]), w);
+            if constexpr (PEERS) push_raw4(peers, pushed, e[u], w);
+            stored += DELTA;
+          }
+        }
+        if (!full) {
+          for (int64_t k = e[u]; k < end; ++k) one(k);  // ragged tail of the tensor (one thread)
+        }
+      }
+    }
+  } else {
+    for (int64_t k = begin + threadIdx.x; k < end; k += kThreads) one(k);
+  }
+  if constexpr (DELTA) {
+    if (changed != nullptr) {
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) stored += __shfl_xor_sync(0xffffffffu, stored, o);
+      __syncthreads();
+      if ((threadIdx.x & 31) == 0 && stored) atomicAdd(&stored_in_cta, stored);
+      __syncthreads();
+      if (threadIdx.x == 0 && stored_in_cta) atomicAdd(changed, static_cast<unsigned long long>(stored_in_cta));
+    }
+  }
+}
+
+// ---------------------------------------------------------------- host side
+constexpr int64_t kMaxSide = 1 << 24;
+constexpr int64_t kMaxNumel = int64_t(1) << 33;  // padded 8-element groups are counted in 32 bits
+
+int check_shape(const char* what, int64_t rows, int64_t cols) {
+  if (rows < 1 || cols < 1 || rows > kMaxSide || cols > kMaxSide || rows * ((cols + 7) / 8 * 8) > kMaxNumel)
+    return fail(HA_ERR_INVALID, "%s: matrices of %lld x %lld", what, (long long)rows, (long long)cols);
+  return HA_OK;
+}
+
+// The planes hold fixed-point fp16, so the steps must keep singular values in range: from [0, s] a
+// step reaches at most max |a t + b t^3 + c t^5| (checked where the derivative vanishes and at s).
+int check_steps(const char* what, const ha_ns_params* ns) {
+  if (ns == nullptr) return fail(HA_ERR_INVALID, "%s: NULL Newton-Schulz parameters", what);
+  if (ns->steps < 1 || ns->steps > HA_NS_MAX_STEPS)
+    return fail(HA_ERR_INVALID, "%s: %d steps (1 to %d)", what, ns->steps, HA_NS_MAX_STEPS);
+  if (!(ns->eps >= 1e-30) || !(ns->eps <= 1e30)) return fail(HA_ERR_INVALID, "%s: eps %g (1e-30 to 1e30)", what, ns->eps);
+  double s = 1.0;
+  for (int i = 0; i < ns->steps; ++i) {
+    const double a = ns->coef[3 * i], b = ns->coef[3 * i + 1], c = ns->coef[3 * i + 2];
+    if (!(std::fabs(a) + std::fabs(b) * s * s + std::fabs(c) * s * s * s * s <= 60.0))
+      return fail(HA_ERR_INVALID, "%s: coefficients (%g, %g, %g) of step %d leave the fp16 range", what, a, b, c, i);
+    auto value = [&](double t) { return std::fabs(t * (a + t * t * (b + t * t * c))); };
+    double top = value(s);
+    const double disc = 9 * b * b - 20 * a * c;
+    if (disc >= 0 && c != 0)
+      for (const double sign : {-1.0, 1.0}) {
+        const double q = (-3 * b + sign * std::sqrt(disc)) / (10 * c);
+        if (q > 0 && q < s * s && value(std::sqrt(q)) > top) top = value(std::sqrt(q));
+      }
+    else if (c == 0 && b != 0 && -a / (3 * b) > 0 && -a / (3 * b) < s * s)
+      top = std::fmax(top, value(std::sqrt(-a / (3 * b))));
+    s = top;
+    if (!(s <= 4.0)) return fail(HA_ERR_INVALID, "%s: step %d lets singular values grow to %g", what, i, s);
+  }
+  return HA_OK;
+}
+
+struct Plan {
+  int64_t cap;        // matrices of one pass through the workspace
+  int64_t chunk;      // elements of a partial sum
+  int n_partials;
+  size_t per_matrix;  // workspace bytes, partial sums included
+};
+
+size_t partial_bytes(int64_t numel) {
+  const int64_t chunk = chunk_for(numel);
+  return size_t(((numel + chunk - 1) / chunk * 8 + 255) / 256 * 256);
+}
+
+int make_plan(const char* what, int64_t n, int64_t rows, int64_t cols, void* ws, size_t bytes, Plan* p) {
+  const int64_t numel = rows * cols;
+  p->chunk = chunk_for(numel);
+  p->n_partials = int((numel + p->chunk - 1) / p->chunk);
+  p->per_matrix = size_t(ns_bytes_per_matrix(rows, cols)) + partial_bytes(numel);
+  if (ws == nullptr || (reinterpret_cast<uintptr_t>(ws) & 255) != 0)
+    return fail(HA_ERR_INVALID, "%s: workspace must be 256-byte aligned", what);
+  if (bytes < kHeader + p->per_matrix)
+    return fail(HA_ERR_INVALID, "%s: workspace of %zu bytes; one matrix needs %zu", what, bytes, kHeader + p->per_matrix);
+  const int64_t fit = int64_t((bytes - kHeader) / p->per_matrix);
+  p->cap = n < fit ? n : fit;
+  if (p->cap > 32768) p->cap = 32768;  // grid.y of the element-wise kernels
+  return HA_OK;
+}
+
+void carve(NsBatch* b, const Plan& p, void* ws, int64_t n, int64_t rows, int64_t cols, double** partials) {
+  char* base = static_cast<char*>(ws);
+  *b = NsBatch{};
+  b->n = n;
+  b->rows = rows;
+  b->cols = cols;
+  b->error = reinterpret_cast<uint32_t*>(base);
+  *partials = reinterpret_cast<double*>(base + kHeader);
+  ns_carve(b, base + kHeader + size_t(p.cap) * partial_bytes(rows * cols));
+}
+
+unsigned load_grid(const NsBatch& b) {
+  return unsigned((b.rows * b.ld_x + kLoadChunk - 1) / kLoadChunk);
+}
+
+template <int DT>
+int orthogonalize(const void* src, void* dst, int64_t batch, int64_t rows, int64_t cols, const ha_ns_params& ns,
+                  const Plan& p, void* ws, cudaStream_t st) {
+  using raw = typename Elem<DT>::raw;
+  const int64_t numel = rows * cols;
+  for (int64_t i = 0; i < batch; i += p.cap) {
+    const int64_t n = batch - i < p.cap ? batch - i : p.cap;
+    NsBatch b;
+    double* partials;
+    carve(&b, p, ws, n, rows, cols, &partials);
+    const raw* x = static_cast<const raw*>(src) + i * numel;
+    const Shape sh{rows, cols, b.ld_x, b.plane_x};
+    square_sum_kernel<DT><<<dim3(unsigned(p.n_partials), unsigned(n)), kThreads, 0, st>>>(
+        x, numel, p.chunk, partials, i == 0 ? b.error : nullptr);
+    load_kernel<<<dim3(load_grid(b), unsigned(n)), kThreads, 0, st>>>(PlainSource<DT>{x, numel}, sh, p.n_partials,
+                                                                     partials, ns.eps, 0, b.hi[0], b.lo);
+    int rc = check_launch("ha_orthogonalize (load)");
+    int at = 0;
+    if (rc == HA_OK) rc = ns_run(b, ns.coef, ns.steps, &at, st);
+    if (rc != HA_OK) return rc;
+    store_kernel<<<dim3(load_grid(b), unsigned(n)), kThreads, 0, st>>>(
+        b.hi[at], sh, static_cast<uint16_t*>(dst) + i * numel, b.error);
+    rc = check_launch("ha_orthogonalize (store)");
+    if (rc != HA_OK) return rc;
+  }
+  return HA_OK;
+}
+
+template <int DT>
+void launch_apply(dim3 grid, cudaStream_t st, const Slice& s, const __half* x, const Shape& sh, int first,
+                  int use_decay, bool delta, const Peers& peers, unsigned long long* changed, const uint32_t* error,
+                  uint32_t* status) {
+  if constexpr (DT != HA_F32) {
+    if (delta) {
+      if (peers.n > 0)
+        apply_kernel<DT, true, true><<<grid, kThreads, 0, st>>>(s, x, sh, first, use_decay, peers, changed, error, status);
+      else
+        apply_kernel<DT, false, true><<<grid, kThreads, 0, st>>>(s, x, sh, first, use_decay, peers, changed, error, status);
+      return;
+    }
+  }
+  if (peers.n > 0)
+    apply_kernel<DT, true, false><<<grid, kThreads, 0, st>>>(s, x, sh, first, use_decay, peers, changed, error, status);
+  else
+    apply_kernel<DT, false, false><<<grid, kThreads, 0, st>>>(s, x, sh, first, use_decay, peers, changed, error, status);
+}
+
+template <int DT>
+int muon_step(const ha_tensor* t, int64_t n, int64_t rows, int64_t cols, const MuonConst& c, const ha_ns_params& ns,
+              bool delta, const Peers& peers, unsigned long long* changed, uint32_t* status, const Plan& p, void* ws,
+              cudaStream_t st) {
+  int64_t next = 0;  // entries looked at
+  bool fresh = true;
+  while (next < n) {
+    // the entries of this pass: those with a gradient, as many as the workspace holds
+    const int64_t begin = next;
+    int64_t count = 0;
+    for (; next < n && count < p.cap; ++next) count += t[next].grad != 0;
+    if (count == 0) break;
+    NsBatch b;
+    double* partials;
+    carve(&b, p, ws, count, rows, cols, &partials);
+    const Shape sh{rows, cols, b.ld_x, b.plane_x};
+    int at = 0;
+    for (int stage = 0; stage < 2; ++stage) {  // momentum and load; then, after the products, the weights
+      MuonSource<DT> src;
+      src.c = c;
+      int64_t k = begin, first = 0;
+      while (first < count) {
+        int m = 0;
+        for (; k < next && m < kSlice; ++k)
+          if (t[k].grad != 0) src.s.t[m++] = t[k];
+        if (stage == 0) {
+          double* part = partials + first * p.n_partials;
+          momentum_kernel<DT><<<dim3(unsigned(p.n_partials), unsigned(m)), kThreads, 0, st>>>(
+              src.s, c, p.chunk, part, fresh ? b.error : nullptr);
+          load_kernel<<<dim3(load_grid(b), unsigned(m)), kThreads, 0, st>>>(src, sh, p.n_partials, part, ns.eps,
+                                                                           int(first), b.hi[0], b.lo);
+          fresh = false;
+        } else {
+          launch_apply<DT>(dim3(unsigned((rows * cols + kApplyChunk - 1) / kApplyChunk), unsigned(m)), st, src.s,
+                           b.hi[at], sh, int(first), c.use_decay, delta, peers, changed, b.error, status);
+        }
+        if (int rc = check_launch(stage == 0 ? "ha_muon_step (momentum)" : "ha_muon_step (weights)")) return rc;
+        first += m;
+      }
+      if (stage == 0)
+        if (int rc = ns_run(b, ns.coef, ns.steps, &at, st)) return rc;
+    }
+  }
+  return HA_OK;
+}
+
+}  // namespace
+}  // namespace ha
+
+extern "C" int ha_orthogonalize_workspace(int64_t batch, int64_t rows, int64_t cols, size_t* out) {
+  using namespace ha;
+  if (out == nullptr) return fail(HA_ERR_INVALID, "ha_orthogonalize_workspace: NULL output");
+  if (batch < 0) return fail(HA_ERR_INVALID, "ha_orthogonalize_workspace: batch %lld", (long long)batch);
+  if (int rc = check_shape("ha_orthogonalize_workspace", rows, cols)) return rc;
+  const size_t one = size_t(ns_bytes_per_matrix(rows, cols)) + partial_bytes(rows * cols);
+  if (size_t(batch) > (SIZE_MAX - kHeader) / one)
+    return fail(HA_ERR_INVALID, "ha_orthogonalize_workspace: batch %lld", (long long)batch);
+  *out = kHeader + size_t(batch > 0 ? batch : 1) * one;
+  return HA_OK;
+}
+
+extern "C" int ha_orthogonalize(const void* src, int src_dtype, void* dst, int64_t batch, int64_t rows, int64_t cols,
+                                const ha_ns_params* ns, void* workspace, size_t workspace_bytes, void* stream) {
+  HA_NVTX_RANGE();
+  using namespace ha;
+  if (!valid_float_dtype(src_dtype)) return fail(HA_ERR_UNSUPPORTED, "ha_orthogonalize: dtype %d", src_dtype);
+  if (batch < 0) return fail(HA_ERR_INVALID, "ha_orthogonalize: batch %lld", (long long)batch);
+  if (int rc = check_shape("ha_orthogonalize", rows, cols)) return rc;
+  if (int rc = check_steps("ha_orthogonalize", ns)) return rc;
+  if (batch == 0) return HA_OK;
+  if (src == nullptr || dst == nullptr) return fail(HA_ERR_INVALID, "ha_orthogonalize: NULL matrices");
+  const uintptr_t elem = src_dtype == HA_F32 ? 4 : 2;
+  if ((reinterpret_cast<uintptr_t>(src) % elem) != 0 || (reinterpret_cast<uintptr_t>(dst) & 1) != 0)
+    return fail(HA_ERR_INVALID, "ha_orthogonalize: misaligned matrices");
+  Plan p;
+  if (int rc = make_plan("ha_orthogonalize", batch, rows, cols, workspace, workspace_bytes, &p)) return rc;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  switch (src_dtype) {
+    case HA_F32: return orthogonalize<HA_F32>(src, dst, batch, rows, cols, *ns, p, workspace, st);
+    case HA_BF16: return orthogonalize<HA_BF16>(src, dst, batch, rows, cols, *ns, p, workspace, st);
+    default: return orthogonalize<HA_F16>(src, dst, batch, rows, cols, *ns, p, workspace, st);
+  }
+}
+
+extern "C" int ha_muon_step(const ha_tensor* h_tensors, int64_t n, int64_t rows, int64_t cols, int grad_dtype,
+                            const ha_muon_scalars* sc, const ha_ns_params* ns, int changed_only, const ha_peers* peers,
+                            unsigned long long* d_changed_groups, uint32_t* d_status, void* workspace,
+                            size_t workspace_bytes, void* stream) {
+  HA_NVTX_RANGE();
+  using namespace ha;
+  if (!valid_float_dtype(grad_dtype)) return fail(HA_ERR_UNSUPPORTED, "ha_muon_step: grad dtype %d", grad_dtype);
+  if (n < 0) return fail(HA_ERR_INVALID, "ha_muon_step: %lld tensors", (long long)n);
+  if (sc == nullptr) return fail(HA_ERR_INVALID, "ha_muon_step: NULL scalars");
+  if (int rc = check_shape("ha_muon_step", rows, cols)) return rc;
+  if (int rc = check_steps("ha_muon_step", ns)) return rc;
+  Peers q{};
+  if (peers != nullptr) {
+    if (peers->n < 0 || peers->n > HA_MAX_PEERS) return fail(HA_ERR_INVALID, "ha_muon_step: %d peers", peers->n);
+    q.n = peers->n;
+    for (int i = 0; i < peers->n; ++i) {
+      if ((peers->delta[i] & 15) != 0)
+        return fail(HA_ERR_INVALID, "ha_muon_step: peer %d offset not 16-byte aligned", i);
+      q.delta[i] = peers->delta[i];
+    }
+  }
+  if (n == 0) return HA_OK;
+  if (h_tensors == nullptr) return fail(HA_ERR_INVALID, "ha_muon_step: NULL table");
+  const uint64_t elem = grad_dtype == HA_F32 ? 3 : 1;
+  for (int64_t i = 0; i < n; ++i) {
+    const ha_tensor& t = h_tensors[i];
+    if (t.grad == 0) continue;
+    if (t.numel != rows * cols || t.master == 0 || t.exp_avg == 0 || (grad_dtype != HA_F32 && t.param == 0))
+      return fail(HA_ERR_INVALID, "ha_muon_step: entry %lld: %lld elements for %lld x %lld, or a NULL address",
+                  (long long)i, (long long)t.numel, (long long)rows, (long long)cols);
+    if (((t.grad | t.param) & elem) != 0 || ((t.master | t.exp_avg) & 3) != 0)
+      return fail(HA_ERR_INVALID, "ha_muon_step: entry %lld: misaligned address", (long long)i);
+  }
+  Plan p;
+  if (int rc = make_plan("ha_muon_step", n, rows, cols, workspace, workspace_bytes, &p)) return rc;
+  const MuonConst c{sc->mu, sc->one_minus_mu, sc->nesterov, sc->use_decay, sc->clip, sc->clip_mult};
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const bool delta = changed_only != 0 && grad_dtype != HA_F32;
+  switch (grad_dtype) {
+    case HA_F32:
+      return muon_step<HA_F32>(h_tensors, n, rows, cols, c, *ns, delta, q, d_changed_groups, d_status, p, workspace, st);
+    case HA_BF16:
+      return muon_step<HA_BF16>(h_tensors, n, rows, cols, c, *ns, delta, q, d_changed_groups, d_status, p, workspace, st);
+    default:
+      return muon_step<HA_F16>(h_tensors, n, rows, cols, c, *ns, delta, q, d_changed_groups, d_status, p, workspace, st);
+  }
+}

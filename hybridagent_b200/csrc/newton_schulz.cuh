@@ -1,0 +1,37 @@
+// Newton-Schulz products on the tensor cores: what muon.cu needs of newton_schulz.cu.
+#pragma once
+
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "hybridagent_b200.h"
+
+namespace ha {
+
+// Fixed-point scales of the 16-bit planes (powers of two, so they cost no rounding): an element of
+// X is at most its largest singular value and starts near 1 / sqrt(rows * cols); fp16 holds
+// normal numbers from 2^-14 up to 65504.
+constexpr float kScaleX = 4096.0f;   // X planes hold 2^12 x
+constexpr float kScaleG = 1024.0f;   // Gram and polynomial planes hold 2^10 times theirs
+constexpr float kScaleLo = 2048.0f;  // the low plane holds 2^11 (2^12 x - high plane)
+
+// A batch of `n` matrices of one shape in workspace.  Rows are padded to 8 elements.
+struct NsBatch {
+  int64_t n, rows, cols;
+  int64_t ld_x, ld_g, m;         // padded row lengths; m = min(rows, cols)
+  int64_t plane_x, plane_g;      // elements of one matrix
+  __half *hi[2], *lo, *gram, *poly;
+  uint32_t* error;               // set to 1 if a wait ran out
+};
+
+// Bytes that one matrix takes (a multiple of 256).
+int64_t ns_bytes_per_matrix(int64_t rows, int64_t cols);
+// Fixed bytes in front (error word, partial sums of `partials` doubles for each matrix are extra).
+void ns_carve(NsBatch* b, void* base);
+
+// Runs `steps` Newton-Schulz steps on hi[0] (+ lo); returns in *out the index of the hi plane that
+// holds the result.
+int ns_run(const NsBatch& b, const float* coef, int steps, int* out, cudaStream_t st);
+
+}  // namespace ha

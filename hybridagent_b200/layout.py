@@ -40,12 +40,13 @@ def greedy_owners(numels: list[int], world: int) -> list[int]:
 
 @dataclass
 class DtypeClass:
-    """All tensors of one parameter dtype and their owner-major slots."""
+    """All tensors of one parameter dtype and update rule, and their owner-major slots."""
     code: int                                   # HA_F32 / HA_BF16 / HA_F16
     indices: list[int]                          # global tensor indices, in list order
     offset: dict[int, int] = field(default_factory=dict)   # index -> element offset in its owner's segment
     seg_len: int = 0                            # elements per rank segment
     own_len: list[int] = field(default_factory=list)       # padded elements used in each rank's segment
+    muon: bool = False                          # matrices that ZeroOneMuon updates
 
     def owned(self, owner: list[int], rank: int) -> list[int]:
         return [i for i in self.indices if owner[i] == rank]
@@ -65,11 +66,12 @@ class Plan:
         return out
 
 
-def plan(numels: list[int], dtype_codes: list[int], world: int) -> Plan:
+def plan(numels: list[int], dtype_codes: list[int], world: int, muon: list[bool] | None = None) -> Plan:
     owner = greedy_owners(numels, world)
+    kinds = list(zip(dtype_codes, [bool(x) for x in muon] if muon is not None else [False] * len(dtype_codes)))
     classes: list[DtypeClass] = []
-    for code in sorted(set(dtype_codes)):
-        cls = DtypeClass(code, [i for i, c in enumerate(dtype_codes) if c == code])
+    for kind in sorted(set(kinds)):
+        cls = DtypeClass(kind[0], [i for i, k in enumerate(kinds) if k == kind], muon=kind[1])
         fill = [0] * world
         for i in cls.indices:
             r = owner[i]

@@ -165,6 +165,7 @@ class _Class:
         self.code = cls.code
         self.dtype = _TORCH[cls.code]
         self.layout = cls
+        self.muon = cls.muon  # matrices of ZeroOneMuon: no exp_avg_sq, updated by ha_muon_step
         self.owned = cls.owned(opt.owner, opt.rank)
         dev = opt.device
         W, r = opt.world, opt.rank
@@ -189,13 +190,14 @@ class _Class:
         # --- fp32 state of the owned tensors
         own_len = max(cls.own_len[r], layout.ALIGN)
         self.exp_avg_buf = torch.zeros(own_len, dtype=torch.float32, device=dev)
-        self.exp_avg_sq_buf = torch.zeros(own_len, dtype=torch.float32, device=dev)
+        self.exp_avg_sq_buf = None if self.muon else torch.zeros(own_len, dtype=torch.float32, device=dev)
         self.master_buf = None if self.code == HA_F32 else torch.empty(own_len, dtype=torch.float32, device=dev)
         for i in self.owned:
             p = opt.params[i]
             o = cls.offset[i]
             opt.exp_avg[i] = self.exp_avg_buf[o:o + numel[i]].view(p.shape)
-            opt.exp_avg_sq[i] = self.exp_avg_sq_buf[o:o + numel[i]].view(p.shape)
+            if not self.muon:
+                opt.exp_avg_sq[i] = self.exp_avg_sq_buf[o:o + numel[i]].view(p.shape)
             if self.code == HA_F32:
                 opt.master[i] = p.data  # optimizer.py:71-73: the fp32 parameter is the master
                 opt.master_is_parameter[i] = True
@@ -209,7 +211,7 @@ class _Class:
         for k, i in enumerate(self.owned):
             tab[k]["master"] = opt.master[i].data_ptr()
             tab[k]["exp_avg"] = opt.exp_avg[i].data_ptr()
-            tab[k]["exp_avg_sq"] = opt.exp_avg_sq[i].data_ptr()
+            tab[k]["exp_avg_sq"] = 0 if self.muon else opt.exp_avg_sq[i].data_ptr()
             tab[k]["param"] = 0 if self.code == HA_F32 else opt.params[i].data_ptr()
             tab[k]["numel"] = numel[i]
         owned_numels = [numel[i] for i in self.owned]
@@ -279,7 +281,7 @@ class _Class:
             # copy-engine all-gather: per part of the update, one copy per peer of the part's
             # elements of this rank's segment to the same place in the peer's buffer
             self.gather_parts, self.gather_copies = [], []
-            if opt.gather_mode == "ce" and self.adamw_chunks[1]:
+            if opt.gather_mode == "ce" and self.adamw_chunks[1] and not self.muon:
                 tab = layout.chunk_table([numel[i] for i in self.owned], HA_ADAMW_CHUNK)
                 self.gather_parts = layout.gather_parts(tab, [cls.offset[i] for i in self.owned],
                                                         [numel[i] for i in self.owned], HA_ADAMW_CHUNK,
@@ -321,6 +323,8 @@ class _Class:
 class ZeroOneAdamW:
     """ZeRO-1 AdamW over CUDA parameters (drop-in for hybrid_rl.optimizer.ZeroOneAdamW)."""
 
+    state_format = STATE_FORMAT
+
     def __init__(self, param_groups, *, rank: int, world_size: int, betas=(0.9, 0.999), eps: float = 1e-8,
                  weight_decay: float = 0.0, use_8bit: bool = False, comm_timeout_s: float | None = None,
                  land_grads: bool = False):
@@ -340,22 +344,22 @@ class ZeroOneAdamW:
         if self.world < 1 or not 0 <= self.rank < self.world:
             raise ValueError(f"invalid rank/world {self.rank}/{self.world}")
         self.step_count = 0
-        flat: list[tuple[torch.nn.Parameter, float]] = []
+        flat: list[tuple[torch.nn.Parameter, float, bool]] = []
         seen: set[int] = set()
         for group in param_groups:
             for parameter in group["params"]:
                 if parameter.requires_grad and id(parameter) not in seen:
                     seen.add(id(parameter))
-                    flat.append((parameter, float(group["lr"])))
+                    flat.append((parameter, float(group["lr"]), self._takes_muon(parameter, group)))
         if not flat:
-            raise ValueError("ZeroOneAdamW received no trainable parameters")
+            raise ValueError(f"{type(self).__name__} received no trainable parameters")
         if self.use_8bit:
             raise NotImplementedError("use_8bit (bitsandbytes PagedAdamW8bit) is not provided by hybridagent_b200")
-        self.params = [p for p, _ in flat]
-        self.lrs = [lr for _, lr in flat]
+        self.params = [p for p, _, _ in flat]
+        self.lrs = [lr for _, lr, _ in flat]
         self.device = self.params[0].device
         if self.device.type != "cuda":
-            raise RuntimeError(f"hybridagent_b200.ZeroOneAdamW runs on CUDA devices only; parameters are on "
+            raise RuntimeError(f"hybridagent_b200.{type(self).__name__} runs on CUDA devices only; parameters are on "
                                f"{self.device} (there is no CPU path)")
         for p in self.params:
             if p.device != self.device:
@@ -367,7 +371,8 @@ class ZeroOneAdamW:
         _lib.lib()  # fail loudly now if the CUDA library is missing
         self._numels = [p.numel() for p in self.params]
         with torch.cuda.device(self.device):
-            self._plan = layout.plan(self._numels, [_CODES[p.dtype] for p in self.params], self.world)
+            self._plan = layout.plan(self._numels, [_CODES[p.dtype] for p in self.params], self.world,
+                                     [muon for _, _, muon in flat])
             self.owner = list(self._plan.owner)
             self.master: dict[int, torch.Tensor] = {}
             self.master_is_parameter: dict[int, bool] = {}
@@ -434,6 +439,10 @@ class ZeroOneAdamW:
             self._setup_landing()
         elif land_grads and self.world == 1:
             self._setup_landing_local()
+
+    def _takes_muon(self, parameter: torch.Tensor, group: dict) -> bool:
+        """Whether a parameter of ``group`` is updated by Muon (ZeroOneMuon)."""
+        return False
 
     def _setup_world(self) -> None:
         """Owners' parameter values to every rank (the reference's broadcast), then the
@@ -674,6 +683,8 @@ class ZeroOneAdamW:
             steps = np.ascontiguousarray(self._steps[idx] + (grad_ptrs != 0))
             _lib.call("ha_fill_step_scalars", len(c.owned), _lib.np_ptr(c.lrs), _lib.np_ptr(steps),
                       self.betas[0], self.betas[1], self.weight_decay, _lib.np_ptr(tab))
+            if c.muon:
+                tab["neg_lr"] = c.neg_lr  # with the shape's factor
         c.table.upload()
 
     def _stage_step(self) -> None:
@@ -1254,16 +1265,17 @@ class ZeroOneAdamW:
                     c.full_run += 1
                     if c.full_run >= 8:  # look again: the learning rate or the gradients may have changed
                         c.delta_next, c.full_run = True, 0
-                if (n and not dense and c.delta_next and c.code != HA_F32 and not ce_gather
-                        and self.comm_mode != "nccl"):
+                changed_only = bool(n and not dense and c.delta_next and c.code != HA_F32 and not ce_gather
+                                    and self.comm_mode != "nccl")
+                if changed_only:
                     _lib.call("ha_memset", c.changed_dev.data_ptr(), 0, 8, self._stream())
+                if n and c.muon:  # (with the copy-engine all-gather too, these store into the peers' copies)
+                    self._update_muon(c, sc, changed_only, p2p)
+                elif changed_only:
                     _lib.call("ha_adamw_step_delta", c.table.ptr, chunks.data_ptr(), n, HA_ADAMW_CHUNK, c.code,
                               ctypes.byref(sc), ctypes.byref(c.peers) if p2p else None, c.changed_dev.data_ptr(),
                               self._stream())
                     self.launches += 1
-                    c.changed_host.copy_(c.changed_dev, non_blocking=True)
-                    c.changed_event = torch.cuda.Event()
-                    c.changed_event.record()
                 elif n and ce_gather:  # update in parts; the copy engines send each finished part to the peers
                     esz = c.packed_param.element_size()
                     for (c0, nc, _, _), copies in zip(c.gather_parts, c.gather_copies):
@@ -1283,6 +1295,10 @@ class ZeroOneAdamW:
                     _lib.call("ha_adamw_step", c.table.ptr, chunks.data_ptr(), n, HA_ADAMW_CHUNK, c.code, c.code,
                               ctypes.byref(sc), self._stream())
                     self.launches += 1
+                if changed_only:
+                    c.changed_host.copy_(c.changed_dev, non_blocking=True)
+                    c.changed_event = torch.cuda.Event()
+                    c.changed_event.record()
             for st in self._gather_streams:
                 main.wait_stream(st)
             self._phase("adamw", False)
@@ -1348,7 +1364,7 @@ class ZeroOneAdamW:
         torch.cuda.current_stream(self.device).synchronize()
         owned = list(self.param_steps)
         return {
-            "format": STATE_FORMAT,
+            "format": self.state_format,
             "world": self.world,
             "rank": self.rank,
             "step_count": self.step_count,
@@ -1361,13 +1377,14 @@ class ZeroOneAdamW:
             "param_steps": {i: int(self._steps[i]) for i in owned},
             "master": {i: self.master[i].detach().to("cpu", copy=True) for i in owned},
             "exp_avg": {i: self.exp_avg[i].detach().to("cpu", copy=True) for i in owned},
-            "exp_avg_sq": {i: self.exp_avg_sq[i].detach().to("cpu", copy=True) for i in owned},
+            "exp_avg_sq": {i: self.exp_avg_sq[i].detach().to("cpu", copy=True) for i in owned
+                           if i in self.exp_avg_sq},
         }
 
     @torch.no_grad()
     def load_state_dict(self, state: dict) -> None:
-        if state.get("format") != STATE_FORMAT:
-            raise ValueError(f"not a {STATE_FORMAT} state dict")
+        if state.get("format") != self.state_format:
+            raise ValueError(f"not a {self.state_format} state dict")
         for key, mine in (("world", self.world), ("rank", self.rank), ("owner", list(self.owner)),
                           ("numels", list(self._numels))):
             if state[key] != mine:
@@ -1375,9 +1392,13 @@ class ZeroOneAdamW:
         owned = list(self.param_steps)
         if sorted(state["param_steps"]) != sorted(owned):
             raise ValueError("state dict holds a different set of owned tensors")
+        if sorted(state["exp_avg_sq"]) != sorted(self.exp_avg_sq):
+            raise ValueError("state dict holds second moments of a different set of tensors")
         for i in owned:
             for name, dst in (("master", self.master[i]), ("exp_avg", self.exp_avg[i]),
-                              ("exp_avg_sq", self.exp_avg_sq[i])):
+                              ("exp_avg_sq", self.exp_avg_sq.get(i))):
+                if dst is None:
+                    continue
                 src = state[name][i]
                 if src.shape != dst.shape:
                     raise ValueError(f"{name}[{i}] has shape {tuple(src.shape)}, expected {tuple(dst.shape)}")

@@ -244,6 +244,56 @@ int ha_adamw_step_delta(const ha_tensor* d_tensors, const ha_chunk* d_chunks, in
                         int param_dtype, const ha_adamw_scalars* sc, const ha_peers* peers,
                         unsigned long long* d_changed_groups, void* stream);
 
+/* ------------------------------------------------------------------ Muon (matrices) */
+
+/* Newton-Schulz steps X <- a X + (b A + c A A) X with A = X X^T (X taken with rows <= cols; a tall
+ * matrix is treated as its transpose), from X = U / max(|U|_F, eps).  Step i uses coef[3i..3i+2] =
+ * (a, b, c).  The products run on fp16 operands with fp32 accumulators; the first three steps keep X
+ * to 22 bits between products.  Steps that could carry a singular value out of fp16's range (above 4,
+ * or |a| + |b| s^2 + |c| s^4 > 60) are refused.  eps is between 1e-30 and 1e30; elements of U far
+ * below 2^-36 eps vanish. */
+#define HA_NS_MAX_STEPS 16
+typedef struct ha_ns_params {
+  int32_t steps;  /* 1 .. HA_NS_MAX_STEPS */
+  int32_t reserved;
+  double eps;
+  float coef[3 * HA_NS_MAX_STEPS];
+} ha_ns_params;
+
+/* Per-launch scalars of the Muon update (host struct). */
+typedef struct ha_muon_scalars {
+  float mu;           /* momentum */
+  float one_minus_mu; /* (float)(1 - mu) */
+  int32_t nesterov;   /* the direction looks ahead: (1 - mu) g + mu M */
+  int32_t use_decay;  /* masters are multiplied by ha_tensor.decay first */
+  int32_t clip;       /* as in ha_adamw_scalars */
+  float clip_mult;
+} ha_muon_scalars;
+
+/* Workspace bytes with which `batch` matrices of rows x cols pass at once (batch 0: one).  The calls
+ * below take any size from that of one matrix up and pass through it several times if they must. */
+int ha_orthogonalize_workspace(int64_t batch, int64_t rows, int64_t cols, size_t* out);
+
+/* Orthogonalises `batch` contiguous row-major matrices of rows x cols: singular values towards 1, singular
+ * vectors kept.  src holds src_dtype (HA_F32 / HA_BF16 / HA_F16), dst receives bf16.  src and dst may
+ * not overlap.  A non-finite element makes its matrix NaN.  workspace: device memory, 256-byte aligned, not
+ * shared with a call that may run at the same time.  Should a wait inside the products run out, dst is NaN. */
+int ha_orthogonalize(const void* src, int src_dtype, void* dst, int64_t batch, int64_t rows, int64_t cols,
+                     const ha_ns_params* ns, void* workspace, size_t workspace_bytes, void* stream);
+
+/* One Muon step of `n` matrices of rows x cols (a HOST table, read before the call returns; entries
+ * with grad == 0 are skipped):
+ *     M <- mu M + (1 - mu) g;  U = direction;  O = Newton-Schulz(U);  W <- W decay + neg_lr O
+ * with M = exp_avg, W = master, and the copy of W in grad_dtype at `param` (16-bit types; for HA_F32
+ * the master is the parameter).  exp_avg_sq, rc1 and rc2 are not read; neg_lr includes any factor for
+ * the shape.  changed_only: 16-bit copies are stored by changed sectors, under ha_adamw_step_delta's
+ * conditions; peers (may be NULL) and d_changed_groups as there.  Should a wait inside the products
+ * run out, the weights stay as they are and *d_status (device, may be NULL) becomes 1. */
+int ha_muon_step(const ha_tensor* h_tensors, int64_t n, int64_t rows, int64_t cols, int grad_dtype,
+                 const ha_muon_scalars* sc, const ha_ns_params* ns, int changed_only, const ha_peers* peers,
+                 unsigned long long* d_changed_groups, uint32_t* d_status, void* workspace, size_t workspace_bytes,
+                 void* stream);
+
 /* ------------------------------------------------------------------ NCCL (NVLink / NVSwitch) */
 
 typedef struct ha_comm ha_comm;
