@@ -248,37 +248,53 @@ __global__ void __launch_bounds__(kThreads) load_kernel(const __grid_constant__ 
   }
 }
 
-// The orthogonalised matrices as bf16 (NaN if a wait of the products ran out).
+// The orthogonalised matrices as bf16 (NaN if a wait of the products ran out), eight elements of the
+// packed result per thread, so that odd row lengths cost unaligned loads but no narrow stores.
 __global__ void __launch_bounds__(kThreads)
-    store_kernel(const __half* x, Shape sh, uint16_t* out, const uint32_t* error) {
+    store_kernel(const __half* x, Shape sh, int64_t total, uint16_t* out, const uint32_t* error) {
   const bool bad = *error != 0;
-  x += int64_t(blockIdx.y) * sh.plane;
-  out += int64_t(blockIdx.y) * sh.rows * sh.cols;
-  const bool vec = (sh.cols & 7) == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
-  const uint32_t per_row = uint32_t(sh.ld >> 3);
-  const int64_t total = sh.rows * per_row;
+  const int64_t numel = sh.rows * sh.cols;
+  const bool vec = (sh.cols & 7) == 0;
 #pragma unroll
   for (int u = 0; u < 4; ++u) {
-    const int64_t k = int64_t(blockIdx.x) * (kThreads * 4) + u * kThreads + threadIdx.x;
-    if (k >= total) break;
-    const uint32_t r = uint32_t(k) / per_row, c = (uint32_t(k) - r * per_row) * 8;
-    const uint4 w = *reinterpret_cast<const uint4*>(x + int64_t(r) * sh.ld + c);
-    const uint32_t v[4] = {w.x, w.y, w.z, w.w};
+    const int64_t e = ((int64_t(blockIdx.x) * 4 + u) * kThreads + threadIdx.x) * 8;
+    if (e >= total) break;
+    int64_t z = e / numel;
+    const int64_t in = e - z * numel;
+    int64_t r = in / sh.cols, c = in - r * sh.cols;
+    const __half* p = x + z * sh.plane + r * sh.ld + c;
     uint32_t b[4];
+    if (vec) {
+      const uint4 w = *reinterpret_cast<const uint4*>(p);
+      b[0] = w.x, b[1] = w.y, b[2] = w.z, b[3] = w.w;
+    } else {
+      uint16_t h[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        h[i] = e + i < total ? __half_as_ushort(*p) : uint16_t(0);
+        ++p;
+        if (++c == sh.cols) {
+          c = 0;
+          if (++r == sh.rows) r = 0, ++z;
+          p = x + z * sh.plane + r * sh.ld;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) b[i] = uint32_t(h[2 * i]) | (uint32_t(h[2 * i + 1]) << 16);
+    }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&v[i]));
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&b[i]));
       b[i] = bad ? 0x7fff7fffu
                  : uint32_t(Elem<HA_BF16>::narrow(f.x * (1.0f / kScaleX))) |
                        (uint32_t(Elem<HA_BF16>::narrow(f.y * (1.0f / kScaleX))) << 16);
     }
-    const int64_t e = int64_t(r) * sh.cols + c;
-    if (vec) {
+    if (e + 8 <= total && (reinterpret_cast<uintptr_t>(out) & 15) == 0) {
       *reinterpret_cast<uint4*>(out + e) = make_uint4(b[0], b[1], b[2], b[3]);
     } else {
 #pragma unroll
       for (int i = 0; i < 8; ++i)
-        if (c + i < sh.cols) out[e + i] = uint16_t(b[i >> 1] >> (16 * (i & 1)));
+        if (e + i < total) out[e + i] = uint16_t(b[i >> 1] >> (16 * (i & 1)));
     }
   }
 }
@@ -417,8 +433,7 @@ int check_shape(const char* what, int64_t rows, int64_t cols) {
   return HA_OK;
 }
 
-// The planes hold fixed-point fp16, so the steps must keep singular values in range: from [0, s] a
-// step reaches at most max |a t + b t^3 + c t^5| (checked where the derivative vanishes and at s).
+// The planes hold scaled fp16, so the steps must keep singular values and factors in range.
 int check_steps(const char* what, const ha_ns_params* ns) {
   if (ns == nullptr) return fail(HA_ERR_INVALID, "%s: NULL Newton-Schulz parameters", what);
   if (ns->steps < 1 || ns->steps > HA_NS_MAX_STEPS)
@@ -426,21 +441,12 @@ int check_steps(const char* what, const ha_ns_params* ns) {
   if (!(ns->eps >= 1e-30) || !(ns->eps <= 1e30)) return fail(HA_ERR_INVALID, "%s: eps %g (1e-30 to 1e30)", what, ns->eps);
   double s = 1.0;
   for (int i = 0; i < ns->steps; ++i) {
-    const double a = ns->coef[3 * i], b = ns->coef[3 * i + 1], c = ns->coef[3 * i + 2];
-    if (!(std::fabs(a) + std::fabs(b) * s * s + std::fabs(c) * s * s * s * s <= 60.0))
-      return fail(HA_ERR_INVALID, "%s: coefficients (%g, %g, %g) of step %d leave the fp16 range", what, a, b, c, i);
-    auto value = [&](double t) { return std::fabs(t * (a + t * t * (b + t * t * c))); };
-    double top = value(s);
-    const double disc = 9 * b * b - 20 * a * c;
-    if (disc >= 0 && c != 0)
-      for (const double sign : {-1.0, 1.0}) {
-        const double q = (-3 * b + sign * std::sqrt(disc)) / (10 * c);
-        if (q > 0 && q < s * s && value(std::sqrt(q)) > top) top = value(std::sqrt(q));
-      }
-    else if (c == 0 && b != 0 && -a / (3 * b) > 0 && -a / (3 * b) < s * s)
-      top = std::fmax(top, value(std::sqrt(-a / (3 * b))));
-    s = top;
-    if (!(s <= 4.0)) return fail(HA_ERR_INVALID, "%s: step %d lets singular values grow to %g", what, i, s);
+    const float* c = ns->coef + 3 * i;
+    if (!(ns_factor(c, s) <= kMaxFactor && std::fabs(c[1]) * s * s <= kMaxFactor && std::fabs(c[2]) * s * s * s * s <= kMaxFactor))
+      return fail(HA_ERR_INVALID, "%s: coefficients (%g, %g, %g) of step %d leave the fp16 range", what, c[0], c[1],
+                  c[2], i);
+    s = ns_growth(c, s);
+    if (!(s <= kMaxGrowth)) return fail(HA_ERR_INVALID, "%s: step %d lets singular values grow to %g", what, i, s);
   }
   return HA_OK;
 }
@@ -507,8 +513,8 @@ int orthogonalize(const void* src, void* dst, int64_t batch, int64_t rows, int64
     int at = 0;
     if (rc == HA_OK) rc = ns_run(b, ns.coef, ns.steps, &at, st);
     if (rc != HA_OK) return rc;
-    store_kernel<<<dim3(load_grid(b), unsigned(n)), kThreads, 0, st>>>(
-        b.hi[at], sh, static_cast<uint16_t*>(dst) + i * numel, b.error);
+    store_kernel<<<dim3(unsigned((n * numel + kLoadChunk - 1) / kLoadChunk)), kThreads, 0, st>>>(
+        b.hi[at], sh, n * numel, static_cast<uint16_t*>(dst) + i * numel, b.error);
     rc = check_launch("ha_orthogonalize (store)");
     if (rc != HA_OK) return rc;
   }

@@ -21,9 +21,16 @@ struct NsBatch {
   int64_t n, rows, cols;
   int64_t ld_x, ld_g, m;         // padded row lengths; m = min(rows, cols)
   int64_t plane_x, plane_g;      // elements of one matrix
-  __half *hi[2], *lo, *gram, *poly;
+  __half *hi[2], *lo;            // X before and after a step; low plane
+  __half* square[3];             // m x m: Gram matrices and factors
   uint32_t* error;               // set to 1 if a wait ran out
 };
+
+// The largest |a t + b t^3 + c t^5| and |a + b t^2 + c t^4| of a step for 0 <= t <= s: how far it can
+// carry singular values up to s, and what it multiplies X by.
+double ns_growth(const float* coef, double s);
+double ns_factor(const float* coef, double s);
+constexpr double kMaxGrowth = 4.0, kMaxFactor = 60.0;  // what the planes hold, with room for rounding
 
 // Bytes that one matrix takes (a multiple of 256).
 int64_t ns_bytes_per_matrix(int64_t rows, int64_t cols);

@@ -249,8 +249,9 @@ int ha_adamw_step_delta(const ha_tensor* d_tensors, const ha_chunk* d_chunks, in
 /* Newton-Schulz steps X <- a X + (b A + c A A) X with A = X X^T (X taken with rows <= cols; a tall
  * matrix is treated as its transpose), from X = U / max(|U|_F, eps).  Step i uses coef[3i..3i+2] =
  * (a, b, c).  The products run on fp16 operands with fp32 accumulators; the first three steps keep X
- * to 22 bits between products.  Steps that could carry a singular value out of fp16's range (above 4,
- * or |a| + |b| s^2 + |c| s^4 > 60) are refused.  eps is between 1e-30 and 1e30; elements of U far
+ * to 22 bits between products.  Steps that could leave fp16's range are refused: with s the largest
+ * singular value a step can meet, |a s + b s^3 + c s^5| up to 4 and |a + b s^2 + c s^4|, |b| s^2 and
+ * |c| s^4 up to 60.  eps is between 1e-30 and 1e30; elements of U far
  * below 2^-36 eps vanish. */
 #define HA_NS_MAX_STEPS 16
 typedef struct ha_ns_params {
