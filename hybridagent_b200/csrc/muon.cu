@@ -30,7 +30,8 @@ constexpr int64_t kMaxPartials = 512;    // partial sums of one matrix at most
 constexpr int kLoadChunk = kThreads * 8 * 4;  // padded elements of a CTA of the load and store kernels
 constexpr int64_t kApplyChunk = 16384;
 constexpr int kGroups = 4;               // 4-element groups per thread and pass of the weight kernel
-constexpr size_t kHeader = 256;          // the workspace's error word
+constexpr int64_t kMaxPass = 32768;      // matrices of one pass: grid.y of the element-wise kernels
+constexpr size_t kHeader = 256;          // the workspace's error word, in front of the matrices' counters
 
 struct Slice {
   ha_tensor t[kSlice];
@@ -206,7 +207,8 @@ struct MuonSource {
 template <class Source>
 __global__ void __launch_bounds__(kThreads) load_kernel(const __grid_constant__ Source src, Shape sh, int n_partials,
                                                         const double* partials, double eps, int first, __half* hi,
-                                                        __half* lo) {
+                                                        __half* lo, uint32_t* counter) {
+  if (blockIdx.x == 0 && threadIdx.x == 0) counter[first + blockIdx.y] = 0;
   __shared__ double red[kThreads / 32];
   const double* part = partials + int64_t(blockIdx.y) * n_partials;
   double sum = 0.0;
@@ -455,26 +457,35 @@ struct Plan {
   int64_t cap;        // matrices of one pass through the workspace
   int64_t chunk;      // elements of a partial sum
   int n_partials;
-  size_t per_matrix;  // workspace bytes, partial sums included
 };
+
+// Workspace: the header, counters of `cap` matrices, their partial sums, their planes.
+size_t counter_bytes(int64_t cap) { return size_t((cap * 4 + 255) / 256 * 256); }
 
 size_t partial_bytes(int64_t numel) {
   const int64_t chunk = chunk_for(numel);
   return size_t(((numel + chunk - 1) / chunk * 8 + 255) / 256 * 256);
 }
 
+size_t workspace_for(int64_t n, int64_t rows, int64_t cols) {
+  return kHeader + counter_bytes(n) + size_t(n) * (size_t(ns_bytes_per_matrix(rows, cols)) + partial_bytes(rows * cols));
+}
+
 int make_plan(const char* what, int64_t n, int64_t rows, int64_t cols, void* ws, size_t bytes, Plan* p) {
   const int64_t numel = rows * cols;
   p->chunk = chunk_for(numel);
   p->n_partials = int((numel + p->chunk - 1) / p->chunk);
-  p->per_matrix = size_t(ns_bytes_per_matrix(rows, cols)) + partial_bytes(numel);
+  const size_t each = size_t(ns_bytes_per_matrix(rows, cols)) + partial_bytes(numel);
   if (ws == nullptr || (reinterpret_cast<uintptr_t>(ws) & 255) != 0)
     return fail(HA_ERR_INVALID, "%s: workspace must be 256-byte aligned", what);
-  if (bytes < kHeader + p->per_matrix)
-    return fail(HA_ERR_INVALID, "%s: workspace of %zu bytes; one matrix needs %zu", what, bytes, kHeader + p->per_matrix);
-  const int64_t fit = int64_t((bytes - kHeader) / p->per_matrix);
-  p->cap = n < fit ? n : fit;
-  if (p->cap > 32768) p->cap = 32768;  // grid.y of the element-wise kernels
+  if (bytes < workspace_for(1, rows, cols))
+    return fail(HA_ERR_INVALID, "%s: workspace of %zu bytes; one matrix needs %zu", what, bytes,
+                workspace_for(1, rows, cols));
+  int64_t cap = n < kMaxPass ? n : kMaxPass;
+  const int64_t fit = int64_t((bytes - kHeader) / each);
+  if (fit < cap) cap = fit;
+  while (cap > 1 && workspace_for(cap, rows, cols) > bytes) --cap;  // (the counters' share: few rounds)
+  p->cap = cap;
   return HA_OK;
 }
 
@@ -485,8 +496,10 @@ void carve(NsBatch* b, const Plan& p, void* ws, int64_t n, int64_t rows, int64_t
   b->rows = rows;
   b->cols = cols;
   b->error = reinterpret_cast<uint32_t*>(base);
-  *partials = reinterpret_cast<double*>(base + kHeader);
-  ns_carve(b, base + kHeader + size_t(p.cap) * partial_bytes(rows * cols));
+  b->counter = reinterpret_cast<uint32_t*>(base + kHeader);
+  base += kHeader + counter_bytes(p.cap);
+  *partials = reinterpret_cast<double*>(base);
+  ns_carve(b, base + size_t(p.cap) * partial_bytes(rows * cols));
 }
 
 unsigned load_grid(const NsBatch& b) {
@@ -508,7 +521,7 @@ int orthogonalize(const void* src, void* dst, int64_t batch, int64_t rows, int64
     square_sum_kernel<DT><<<dim3(unsigned(p.n_partials), unsigned(n)), kThreads, 0, st>>>(
         x, numel, p.chunk, partials, i == 0 ? b.error : nullptr);
     load_kernel<<<dim3(load_grid(b), unsigned(n)), kThreads, 0, st>>>(PlainSource<DT>{x, numel}, sh, p.n_partials,
-                                                                     partials, ns.eps, 0, b.hi[0], b.lo);
+                                                                     partials, ns.eps, 0, b.hi[0], b.lo, b.counter);
     int rc = check_launch("ha_orthogonalize (load)");
     int at = 0;
     if (rc == HA_OK) rc = ns_run(b, ns.coef, ns.steps, &at, st);
@@ -570,7 +583,8 @@ int muon_step(const ha_tensor* t, int64_t n, int64_t rows, int64_t cols, const M
           momentum_kernel<DT><<<dim3(unsigned(p.n_partials), unsigned(m)), kThreads, 0, st>>>(
               src.s, c, p.chunk, part, fresh ? b.error : nullptr);
           load_kernel<<<dim3(load_grid(b), unsigned(m)), kThreads, 0, st>>>(src, sh, p.n_partials, part, ns.eps,
-                                                                           int(first), b.hi[0], b.lo);
+                                                                           int(first), b.hi[0], b.lo,
+                                                                           b.counter);
           fresh = false;
         } else {
           launch_apply<DT>(dim3(unsigned((rows * cols + kApplyChunk - 1) / kApplyChunk), unsigned(m)), st, src.s,
@@ -594,10 +608,8 @@ extern "C" int ha_orthogonalize_workspace(int64_t batch, int64_t rows, int64_t c
   if (out == nullptr) return fail(HA_ERR_INVALID, "ha_orthogonalize_workspace: NULL output");
   if (batch < 0) return fail(HA_ERR_INVALID, "ha_orthogonalize_workspace: batch %lld", (long long)batch);
   if (int rc = check_shape("ha_orthogonalize_workspace", rows, cols)) return rc;
-  const size_t one = size_t(ns_bytes_per_matrix(rows, cols)) + partial_bytes(rows * cols);
-  if (size_t(batch) > (SIZE_MAX - kHeader) / one)
-    return fail(HA_ERR_INVALID, "ha_orthogonalize_workspace: batch %lld", (long long)batch);
-  *out = kHeader + size_t(batch > 0 ? batch : 1) * one;
+  const int64_t n = batch < 1 ? 1 : (batch > kMaxPass ? kMaxPass : batch);
+  *out = workspace_for(n, rows, cols);
   return HA_OK;
 }
 

@@ -23,6 +23,7 @@ struct NsBatch {
   int64_t plane_x, plane_g;      // elements of one matrix
   __half *hi[2], *lo;            // X before and after a step; low plane
   __half* square[3];             // m x m: Gram matrices and factors
+  uint32_t* counter;             // one for each matrix, zero before the run
   uint32_t* error;               // set to 1 if a wait ran out
 };
 
@@ -34,7 +35,7 @@ constexpr double kMaxGrowth = 4.0, kMaxFactor = 60.0;  // what the planes hold, 
 
 // Bytes that one matrix takes (a multiple of 256).
 int64_t ns_bytes_per_matrix(int64_t rows, int64_t cols);
-// Fixed bytes in front (error word, partial sums of `partials` doubles for each matrix are extra).
+// Lays the planes of b->n matrices out from `base` on.
 void ns_carve(NsBatch* b, void* base);
 
 // Runs `steps` Newton-Schulz steps on hi[0] (+ lo); returns in *out the index of the hi plane that

@@ -70,11 +70,6 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 
-// Programmatic dependent launch: lets the next kernel of the stream start its prologue, and waits
-// until the kernels before this one have finished and their writes are visible.
-__device__ __forceinline__ void grid_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-__device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-
 // Bounded wait: false once `kWaitNs` have passed, or as soon as another thread of the CTA gave up
 // (*stop).  No wait of a healthy launch comes near the limit: it is some hundred times the longest
 // kernel; it turns a lost arrival into an error word instead of a GPU that never answers.
@@ -92,6 +87,57 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
       return false;
     }
   }
+}
+
+// The same for a counter in global memory that other CTAs of the launch raise: true once it has
+// reached `want`, with everything they wrote before raising it visible, to TMA too.
+__device__ __forceinline__ uint32_t load_acquire(const uint32_t* p) {
+  uint32_t v;
+  asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
+  return v;
+}
+__device__ __forceinline__ bool counter_wait(const uint32_t* counter, uint32_t want, volatile uint32_t* stop) {
+  if (load_acquire(counter) < want) {
+    const uint64_t t0 = global_ns();
+    for (;;) {
+      bool done = false;
+#pragma unroll 1
+      for (int i = 0; i < 256 && !done; ++i) done = load_acquire(counter) >= want;
+      if (done) break;
+      if (*stop) return false;
+      if (global_ns() - t0 > kWaitNs) {
+        *stop = 1;
+        return false;
+      }
+    }
+  }
+  asm volatile("fence.proxy.async;" ::: "memory");
+  return true;
+}
+// What one thread of a CTA has waited for with counter_wait, passed on to another through shared memory.
+__device__ __forceinline__ void grant(uint32_t* granted, uint32_t value) {
+  asm volatile("st.release.cta.shared::cta.u32 [%0], %1;" ::"r"(smem_u32(granted)), "r"(value) : "memory");
+}
+__device__ __forceinline__ bool granted_wait(uint32_t* granted, uint32_t want, volatile uint32_t* stop) {
+  const uint64_t t0 = global_ns();
+  for (uint32_t i = 1;; ++i) {
+    uint32_t v;
+    asm volatile("ld.acquire.cta.shared::cta.u32 %0, [%1];" : "=r"(v) : "r"(smem_u32(granted)) : "memory");
+    if (v >= want) break;
+    if ((i & 255) == 0) {
+      if (*stop) return false;
+      if (global_ns() - t0 > kWaitNs) {
+        *stop = 1;
+        return false;
+      }
+    }
+  }
+  asm volatile("fence.proxy.async;" ::: "memory");
+  return true;
+}
+// Raises it after this thread's TMA stores, which have completed.
+__device__ __forceinline__ void counter_raise(uint32_t* counter) {
+  asm volatile("red.release.gpu.global.add.u32 [%0], 1;" ::"l"(counter) : "memory");
 }
 
 // ---------------------------------------------------------------- TMA

@@ -271,7 +271,7 @@ typedef struct ha_muon_scalars {
   float clip_mult;
 } ha_muon_scalars;
 
-/* Workspace bytes with which `batch` matrices of rows x cols pass at once (batch 0: one).  The calls
+/* Workspace bytes with which `batch` matrices of rows x cols (at most 32768 of them) pass at once.  The calls
  * below take any size from that of one matrix up and pass through it several times if they must. */
 int ha_orthogonalize_workspace(int64_t batch, int64_t rows, int64_t cols, size_t* out);
 
