@@ -414,7 +414,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) newton_schulz_kernel(const __
         const int kblocks = (g.K + kBK - 1) / kBK;
         const uint32_t idesc = f16_idesc(kTile, kTile, g.a_mn, g.b_mn);
         const uint32_t lead_a = g.a_mn ? 8192 : 16, lead_b = g.b_mn ? 8192 : 16;
-        const int next_a = g.a_mn ? 128 : 2, next_b = g.b_mn ? 128 : 2;  // 16 K further, in 16-byte units
+        const uint32_t next_a = g.a_mn ? kStepMN : kStepK, next_b = g.b_mn ? kStepMN : kStepK;
         for (int t = first_tile(g, first, step); t < g.tiles && ok; t += step) {
           ok = mbar_wait(smem_u32(&sh.acc_empty[acc]), acc_phase ^ 1, &sh.stop);
           if (!ok) break;
@@ -425,7 +425,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) newton_schulz_kernel(const __
             if (!ok) break;
             tc_fence_after();
             const uint32_t a = ring + slot * kSlot, b = a + kHalf;
-            const uint64_t da = smem_desc(a, lead_a, 1024), db = smem_desc(b, lead_b, 1024);
+            const uint32_t da = smem_desc(a, lead_a), db = smem_desc(b, lead_b);
 #pragma unroll
             for (int k = 0; k < kBK / 16; ++k)
               mma_f16<CG>(d, da + k * next_a, db + k * next_b, idesc, kb > 0 || k > 0);
@@ -688,6 +688,11 @@ int64_t up(int64_t x, int64_t a) { return (x + a - 1) / a * a; }
 
 }  // namespace
 
+int ns_map(CUtensorMap* map, const __half* plane, const NsBatch& b, int box_cols, int box_rows) {
+  return make_map(map, Operand{plane, b.rows, b.cols, b.ld_x, b.plane_x}, b.n, box_cols, box_rows,
+                  CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
 double ns_growth(const float* c, double s) {
   const double a = c[0], b = c[1], d = c[2];
   auto value = [&](double t) { return std::fabs(t * (a + t * t * (b + t * t * d))); };
@@ -736,6 +741,7 @@ void ns_carve(NsBatch* b, void* base) {
 int ns_run(const NsBatch& b, const float* coef, int steps, int* out, cudaStream_t st) {
   int sms = 0;
   if (int rc = sm_count(&sms)) return rc;
+  if (narrow_fits(b.rows, b.cols, coef, steps)) return narrow_run(b, coef, steps, out, sms, st);
   RunArgs p;
   if (int rc = make_maps(b, &p)) return rc;
   p.counter = b.counter;

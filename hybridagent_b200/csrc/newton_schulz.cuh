@@ -1,6 +1,7 @@
 // Newton-Schulz products on the tensor cores: what muon.cu needs of newton_schulz.cu.
 #pragma once
 
+#include <cuda.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -37,6 +38,13 @@ constexpr double kMaxGrowth = 4.0, kMaxFactor = 60.0;  // what the planes hold, 
 int64_t ns_bytes_per_matrix(int64_t rows, int64_t cols);
 // Lays the planes of b->n matrices out from `base` on.
 void ns_carve(NsBatch* b, void* base);
+
+// Map of X-shaped planes, read or written in box_cols x box_rows pieces (128-byte swizzled rows).
+int ns_map(CUtensorMap* map, const __half* plane, const NsBatch& b, int box_cols, int box_rows);
+
+// Matrices whose shorter side is at most 128, if the steps' factors fit (newton_schulz_narrow.cu).
+bool narrow_fits(int64_t rows, int64_t cols, const float* coef, int steps);
+int narrow_run(const NsBatch& b, const float* coef, int steps, int* out, int sms, cudaStream_t st);
 
 // Runs `steps` Newton-Schulz steps on hi[0] (+ lo); returns in *out the index of the hi plane that
 // holds the result.

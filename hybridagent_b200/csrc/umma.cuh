@@ -200,21 +200,35 @@ __device__ __forceinline__ void tmem_dealloc(uint32_t addr, uint32_t columns) {
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
+// Shared-memory operand descriptor, 128-byte swizzle, tile start aligned to 1024 bytes.
+//   K-major (rows of 64 K-elements = 128 bytes): 8-row groups 1024 bytes apart;
+//     `lead` unused; the next 16 K-elements start 32 bytes further.
+//   MN-major (rows of 64 MN-elements, one row per K-index): 8-K groups 1024 bytes apart,
+//     64-element MN blocks `lead` bytes apart; the next 16 K-indices start 2048 bytes further.
+// Only its low word varies (start address in 16-byte units, `lead`); the high word holds the 1024 bytes,
+// the descriptor's version and the swizzle.  Stepping along K adds to the low word.
+constexpr uint32_t kDescHigh = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t smem_desc(uint32_t addr, uint32_t lead) {
+  return ((addr >> 4) & 0x3fff) | ((lead >> 4) << 16);  // (addresses hold the CTA's rank in a cluster above)
+}
+constexpr uint32_t kStepK = 32 >> 4, kStepMN = 2048 >> 4;  // the next 16 K-indices
+
 // D[tmem] (+)= A * B, both operands 16-bit floats of the type in `idesc`, fp32 accumulators.  CG = 2:
 // issued by the pair's first CTA; each CTA holds its half of A's rows, of B's columns and of D's rows.
+// a, b: low words of the operands' descriptors.
 template <int CG>
-__device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+__device__ __forceinline__ void mma_f16(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool accumulate) {
   if constexpr (CG == 1) {
     asm volatile(
-        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-        " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"(uint32_t(accumulate))
+        "{\n .reg .pred p;\n .reg .b64 x, y;\n setp.ne.b32 p, %4, 0;\n mov.b64 x, {%1, %5};\n mov.b64 y, {%2, %5};\n"
+        " tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, p;\n}\n" ::"r"(d),
+        "r"(a), "r"(b), "r"(idesc), "r"(uint32_t(accumulate)), "r"(kDescHigh)
         : "memory");
   } else {
     asm volatile(
-        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-        " tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"(uint32_t(accumulate))
+        "{\n .reg .pred p;\n .reg .b64 x, y;\n setp.ne.b32 p, %4, 0;\n mov.b64 x, {%1, %5};\n mov.b64 y, {%2, %5};\n"
+        " tcgen05.mma.cta_group::2.kind::f16 [%0], x, y, %3, p;\n}\n" ::"r"(d),
+        "r"(a), "r"(b), "r"(idesc), "r"(uint32_t(accumulate)), "r"(kDescHigh)
         : "memory");
   }
 }
@@ -244,17 +258,6 @@ __device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t (&r)[32]) {
       : "r"(addr));
 }
 __device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
-
-// Shared-memory operand descriptor, 128-byte swizzle, tile start aligned to 1024 bytes.
-//   K-major (rows of 64 K-elements = 128 bytes): 8-row groups 1024 bytes apart (`stride`);
-//     `lead` unused; the next 16 K-elements start 32 bytes further.
-//   MN-major (rows of 64 MN-elements, one row per K-index): 8-K groups 1024 bytes apart
-//     (`stride`), 64-element MN blocks `lead` bytes apart; the next 16 K-indices start
-//     2048 bytes further.
-__device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t lead, uint32_t stride) {
-  return uint64_t((addr >> 4) & 0x3fff) | (uint64_t((lead >> 4) & 0x3fff) << 16) |
-         (uint64_t((stride >> 4) & 0x3fff) << 32) | (1ull << 46) | (2ull << 61);
-}
 
 // Instruction descriptor of kind::f16 with fp16 operands and fp32 accumulators; *_mn: that operand
 // is MN-major.
