@@ -31,6 +31,7 @@ constexpr int kLoadChunk = kThreads * 8 * 4;  // padded elements of a CTA of the
 constexpr int64_t kApplyChunk = 16384;
 constexpr int kGroups = 4;               // 4-element groups per thread and pass of the weight kernel
 constexpr int64_t kMaxPass = 32768;      // matrices of one pass: grid.y of the element-wise kernels
+constexpr int64_t kSliceBytes = 48 << 20;  // of matrices between the two reads of a slice: they stay in L2
 constexpr size_t kHeader = 256;          // the workspace's error word, in front of the matrices' counters
 
 struct Slice {
@@ -518,10 +519,16 @@ int orthogonalize(const void* src, void* dst, int64_t batch, int64_t rows, int64
     carve(&b, p, ws, n, rows, cols, &partials);
     const raw* x = static_cast<const raw*>(src) + i * numel;
     const Shape sh{rows, cols, b.ld_x, b.plane_x};
-    square_sum_kernel<DT><<<dim3(unsigned(p.n_partials), unsigned(n)), kThreads, 0, st>>>(
-        x, numel, p.chunk, partials, i == 0 ? b.error : nullptr);
-    load_kernel<<<dim3(load_grid(b), unsigned(n)), kThreads, 0, st>>>(PlainSource<DT>{x, numel}, sh, p.n_partials,
-                                                                     partials, ns.eps, 0, b.hi[0], b.lo, b.counter);
+    int64_t slice = kSliceBytes / (numel * int64_t(sizeof(raw)));
+    if (slice < 1) slice = 1;
+    for (int64_t k = 0; k < n; k += slice) {
+      const unsigned m = unsigned(n - k < slice ? n - k : slice);
+      double* part = partials + k * p.n_partials;
+      square_sum_kernel<DT><<<dim3(unsigned(p.n_partials), m), kThreads, 0, st>>>(
+          x + k * numel, numel, p.chunk, part, i == 0 && k == 0 ? b.error : nullptr);
+      load_kernel<<<dim3(load_grid(b), m), kThreads, 0, st>>>(PlainSource<DT>{x + k * numel, numel}, sh, p.n_partials, part,
+                                                             ns.eps, int(k), b.hi[0], b.lo, b.counter);
+    }
     int rc = check_launch("ha_orthogonalize (load)");
     int at = 0;
     if (rc == HA_OK) rc = ns_run(b, ns.coef, ns.steps, &at, st);

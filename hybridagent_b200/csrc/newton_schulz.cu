@@ -32,9 +32,9 @@
 // MMAs, and eight epilogue warps read the accumulators from one of two TMEM buffers while the next tile
 // is multiplied.  Results leave in blocks of 128 x 32 through a second ring: warp 2 fetches a block's addend
 // into it, four epilogue warps (one for each quarter of the TMEM lanes; two such groups take turns) replace it by
-// the result, and warp 3 stores it by TMA, which clips the edges, and raises the matrix's counter after a
-// tile's last block.  Fetching, storing and signalling cost a microsecond each, so none is left to the
-// epilogue warps: products with small K are bound by the epilogue.  Tall matrices (rows > cols) are not
+// the result, and a store warp for each group moves it out by TMA, which clips the edges, and raises the
+// matrix's counter after its last block of a tile.  Fetching, storing and signalling take long, so none is left
+// to the epilogue warps: products with small K are bound by the epilogue.  Tall matrices (rows > cols) are not
 // transposed: both operand layouts (K contiguous, or M/N contiguous) are read by the MMA as they lie.
 #include <cuda.h>
 
@@ -49,7 +49,7 @@ namespace {
 
 constexpr int kBM = 128;           // rows of a CTA's part of a tile: the TMEM lanes
 constexpr int kBK = 64;            // K elements of a ring slot: one 128-byte swizzle row
-constexpr int kGemmThreads = 384;  // operands, MMA, addends, stores: a warp each; eight epilogue warps
+constexpr int kGemmThreads = 416;  // operands, MMA, addends, stores; eight epilogue warps; stores
 constexpr int kPreciseSteps = 3;
 constexpr int kHalf = kBM * kBK * 2;  // bytes of one operand's part of a slot
 constexpr int kSlot = 2 * kHalf;
@@ -84,7 +84,7 @@ struct Stage {
   int skew;           // tiles of the stages before, modulo the CTAs (or pairs): the list goes on where it stopped
   uint32_t before;    // a matrix's counter when its previous stage is stored
   int8_t epilogue, m_fast, a_mn, b_mn;  // *_mn: the operand's M / N index is the contiguous one
-  int8_t map_a, map_b, map_out, map_2, map_add;
+  int8_t map_a, map_b, map_out, map_2, map_add, keep_low;
   float scale, add, diag;
 };
 constexpr int kMaxStages = 3 * HA_NS_MAX_STEPS + 2;
@@ -282,36 +282,38 @@ __device__ __forceinline__ void feed_blocks(const RunArgs& p, Shared& sh, uint32
   }
 }
 
-// Warp 3, one thread: finished blocks to memory, and the counters.
+// Warps 3 and 12, one thread each: the blocks that one epilogue group finished, to memory; then the counter.
 template <int CG>
-__device__ __forceinline__ void store_blocks(const RunArgs& p, Shared& sh, uint32_t ring, int first, int step, int rank) {
-  constexpr int kPending = 2;
+__device__ __forceinline__ void store_blocks(const RunArgs& p, Shared& sh, uint32_t ring, int first, int step, int rank,
+                                             uint32_t group) {
   uint32_t n = 0;
   for (int s = 0; s < p.stages; ++s) {
     const Stage& g = p.stage[s];
     for (int t = first_tile(g, first, step); t < g.tiles; t += step) {
       const TileAt at = tile_at(g, t);
       const int blocks = blocks_of<CG>(g, at, rank), row = at.i * (128 * CG) + rank * kBM;
-      for (int k = 0; k < blocks; ++k, ++n) {
-        const uint32_t b = n % kBlocks, block = ring + b * kBlock, second = block + kBlocks * kBlock;
+      uint32_t last = kBlocks;  // block of the store before, not yet handed back
+      for (int k = int((n ^ group) & 1); k < blocks; k += 2) {
+        const uint32_t b = (n + k) % kBlocks, block = ring + b * kBlock, second = block + kBlocks * kBlock;
         const int col = at.j * (128 * CG) + k * kBlockCols;
-        if (!mbar_wait(smem_u32(&sh.blk_ready[b]), (n / kBlocks) & 1, &sh.stop)) return;
+        if (!mbar_wait(smem_u32(&sh.blk_ready[b]), ((n + k) / kBlocks) & 1, &sh.stop)) return;
         if (g.epilogue == kPrecise) {
-          tma_store_3d(&p.map[g.map_2], block, col, row, at.z);
           tma_store_3d(&p.map[g.map_out], second, col, row, at.z);
+          if (g.keep_low) tma_store_3d(&p.map[g.map_2], block, col, row, at.z);
         } else {
           tma_store_3d(&p.map[g.map_out], block, col, row, at.z);
           if (g.epilogue <= kPoly && at.i != at.j) tma_store_3d(&p.map[g.map_2], second, row, col, at.z);
         }
         tma_store_commit();
-        if (k >= kPending) {  // all but the last kPending blocks have been read
-          tma_store_wait_read<kPending>();
-          mbar_arrive(smem_u32(&sh.blk_free[(n - kPending) % kBlocks]));
+        if (last < kBlocks) {
+          tma_store_wait_read<1>();
+          mbar_arrive(smem_u32(&sh.blk_free[last]));
         }
+        last = b;
       }
+      n += blocks;
       tma_store_wait_all();
-      for (int k = blocks < kPending ? blocks : kPending; k > 0; --k)
-        mbar_arrive(smem_u32(&sh.blk_free[(n - k) % kBlocks]));
+      if (last < kBlocks) mbar_arrive(smem_u32(&sh.blk_free[last]));
       counter_raise(p.counter + at.z);
     }
   }
@@ -441,9 +443,9 @@ __global__ void __launch_bounds__(kGemmThreads, 1) newton_schulz_kernel(const __
   } else if (warp == 2) {
     if (lane == 0) feed_blocks<CG>(p, sh, ring + kSlots * kSlot, first, step, int(rank));
     __syncwarp();
-  } else if (warp == 3) {
+  } else if (warp == 3 || warp == 12) {
     if (lane == 0) {
-      store_blocks<CG>(p, sh, ring + kSlots * kSlot, first, step, int(rank));
+      store_blocks<CG>(p, sh, ring + kSlots * kSlot, first, step, int(rank), warp == 3 ? 0 : 1);
       tma_store_wait_all();
     }
     __syncwarp();
@@ -629,6 +631,7 @@ int make_stages(const NsBatch& b, const float* coef, int steps, RunArgs* p) {
     g->scale = 1.0f / kScaleG;
     g->add = (pair ? c[0] * c[3] : c[0]) / kScaleLo;
     s += pair ? 2 : 1;
+    g->keep_low = s < kPreciseSteps && s < steps;  // the next step reads it
   }
   return cur;
 }
@@ -650,7 +653,7 @@ int64_t cut(RunArgs* p, int64_t batch, int cg, int sms) {
     g.m_fast = g.tiles_m <= g.tiles_n;  // the shorter side first: its operand panels stay in L2
     g.skew = int(skew);
     g.before = before;
-    before += uint32_t(per) * cg;  // each CTA of a tile raises it once
+    before += uint32_t(per) * 2 * cg;  // both store warps of each of its CTAs
     skew = (skew + g.tiles) % workers;
     cost += (g.tiles + workers - 1) / workers * cg * ((g.K + kBK - 1) / kBK);
   }
