@@ -96,7 +96,7 @@ SIGNATURES: dict[str, tuple[list, object]] = {
     "ha_orthogonalize_workspace": ([_i64, _i64, _i64, ctypes.POINTER(_sz)], ctypes.c_int),
     "ha_orthogonalize": ([_vp, ctypes.c_int, _vp, _i64, _i64, _i64, ctypes.POINTER(NsParams), _vp, _sz, _vp],
                          ctypes.c_int),
-    "ha_muon_step": ([_vp, _i64, _i64, _i64, ctypes.c_int, ctypes.POINTER(MuonScalars), ctypes.POINTER(NsParams),
+    "ha_muon_step": ([_vp, _vp, _i64, ctypes.c_int, ctypes.POINTER(MuonScalars), ctypes.POINTER(NsParams),
                       ctypes.c_int, ctypes.POINTER(Peers), _vp, _vp, _vp, _sz, _vp], ctypes.c_int),
     "ha_comm_unique_id": ([_vp], ctypes.c_int),
     "ha_comm_init": ([_vp, _i32, _i32, ctypes.POINTER(ctypes.c_void_p)], ctypes.c_int),

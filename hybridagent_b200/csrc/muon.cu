@@ -30,9 +30,9 @@ constexpr int64_t kMaxPartials = 512;    // partial sums of one matrix at most
 constexpr int kLoadChunk = kThreads * 8 * 4;  // padded elements of a CTA of the load and store kernels
 constexpr int64_t kApplyChunk = 16384;
 constexpr int kGroups = 4;               // 4-element groups per thread and pass of the weight kernel
-constexpr int64_t kMaxPass = 32768;      // matrices of one pass: grid.y of the element-wise kernels
+constexpr int64_t kMaxPass = 4096;       // matrices of one pass
 constexpr int64_t kSliceBytes = 48 << 20;  // of matrices between the two reads of a slice: they stay in L2
-constexpr size_t kHeader = 256;          // the workspace's error word, in front of the matrices' counters
+constexpr size_t kHeader = 256 + kMaxPass * 4;  // the workspace's error word, the matrices' counters
 
 struct Slice {
   ha_tensor t[kSlice];
@@ -454,87 +454,98 @@ int check_steps(const char* what, const ha_ns_params* ns) {
   return HA_OK;
 }
 
-struct Plan {
-  int64_t cap;        // matrices of one pass through the workspace
-  int64_t chunk;      // elements of a partial sum
-  int n_partials;
-};
-
-// Workspace: the header, counters of `cap` matrices, their partial sums, their planes.
-size_t counter_bytes(int64_t cap) { return size_t((cap * 4 + 255) / 256 * 256); }
-
 size_t partial_bytes(int64_t numel) {
   const int64_t chunk = chunk_for(numel);
   return size_t(((numel + chunk - 1) / chunk * 8 + 255) / 256 * 256);
 }
-
-size_t workspace_for(int64_t n, int64_t rows, int64_t cols) {
-  return kHeader + counter_bytes(n) + size_t(n) * (size_t(ns_bytes_per_matrix(rows, cols)) + partial_bytes(rows * cols));
+// Workspace of a matrix: its partial sums and planes.
+size_t matrix_bytes(int64_t rows, int64_t cols) {
+  return size_t(ns_bytes_per_matrix(rows, cols)) + partial_bytes(rows * cols);
 }
 
-int make_plan(const char* what, int64_t n, int64_t rows, int64_t cols, void* ws, size_t bytes, Plan* p) {
-  const int64_t numel = rows * cols;
-  p->chunk = chunk_for(numel);
-  p->n_partials = int((numel + p->chunk - 1) / p->chunk);
-  const size_t each = size_t(ns_bytes_per_matrix(rows, cols)) + partial_bytes(numel);
+int check_workspace(const char* what, int64_t rows, int64_t cols, const void* ws, size_t bytes) {
   if (ws == nullptr || (reinterpret_cast<uintptr_t>(ws) & 255) != 0)
     return fail(HA_ERR_INVALID, "%s: workspace must be 256-byte aligned", what);
-  if (bytes < workspace_for(1, rows, cols))
-    return fail(HA_ERR_INVALID, "%s: workspace of %zu bytes; one matrix needs %zu", what, bytes,
-                workspace_for(1, rows, cols));
-  int64_t cap = n < kMaxPass ? n : kMaxPass;
-  const int64_t fit = int64_t((bytes - kHeader) / each);
-  if (fit < cap) cap = fit;
-  while (cap > 1 && workspace_for(cap, rows, cols) > bytes) --cap;  // (the counters' share: few rounds)
-  p->cap = cap;
+  const size_t one = kHeader + matrix_bytes(rows, cols);
+  if (bytes < one) return fail(HA_ERR_INVALID, "%s: workspace of %zu bytes; one matrix needs %zu", what, bytes, one);
   return HA_OK;
 }
 
-void carve(NsBatch* b, const Plan& p, void* ws, int64_t n, int64_t rows, int64_t cols, double** partials) {
-  char* base = static_cast<char*>(ws);
-  *b = NsBatch{};
-  b->n = n;
-  b->rows = rows;
-  b->cols = cols;
-  b->error = reinterpret_cast<uint32_t*>(base);
-  b->counter = reinterpret_cast<uint32_t*>(base + kHeader);
-  base += kHeader + counter_bytes(p.cap);
-  *partials = reinterpret_cast<double*>(base);
-  ns_carve(b, base + size_t(p.cap) * partial_bytes(rows * cols));
-}
+// Matrices of one shape in a pass through the workspace.
+struct Group {
+  NsBatch b;
+  double* partials;
+  int64_t chunk;   // elements of a partial sum
+  int n_partials;
+  int64_t begin;   // first entry of the caller's table
+};
+struct Pass {
+  Group group[kNsShapes];
+  NsBatch batches[kNsShapes];
+  int groups = 0;
+  int64_t matrices = 0;
+  size_t used = kHeader;
+  char* base;
+  explicit Pass(void* ws) : base(static_cast<char*>(ws)) {}
+  // Takes `n` matrices; the caller has checked that they fit.
+  Group& add(int64_t n, int64_t rows, int64_t cols, int64_t begin) {
+    Group& g = group[groups];
+    g = Group{};
+    g.begin = begin;
+    g.chunk = chunk_for(rows * cols);
+    g.n_partials = int((rows * cols + g.chunk - 1) / g.chunk);
+    g.b.n = n;
+    g.b.rows = rows;
+    g.b.cols = cols;
+    g.b.error = reinterpret_cast<uint32_t*>(base);
+    g.b.counter = reinterpret_cast<uint32_t*>(base + 256) + matrices;
+    g.partials = reinterpret_cast<double*>(base + used);
+    ns_carve(&g.b, base + used + size_t(n) * partial_bytes(rows * cols));
+    used += size_t(n) * matrix_bytes(rows, cols);
+    matrices += n;
+    ++groups;
+    return g;
+  }
+  int run(const ha_ns_params& ns, cudaStream_t st) {
+    for (int i = 0; i < groups; ++i) batches[i] = group[i].b;
+    const int rc = ns_run(batches, groups, ns.coef, ns.steps, st);
+    for (int i = 0; i < groups; ++i) group[i].b.out = batches[i].out;
+    return rc;
+  }
+};
 
 unsigned load_grid(const NsBatch& b) {
   return unsigned((b.rows * b.ld_x + kLoadChunk - 1) / kLoadChunk);
 }
 
 template <int DT>
-int orthogonalize(const void* src, void* dst, int64_t batch, int64_t rows, int64_t cols, const ha_ns_params& ns,
-                  const Plan& p, void* ws, cudaStream_t st) {
+int orthogonalize(const void* src, void* dst, int64_t batch, int64_t rows, int64_t cols, const ha_ns_params& ns, void* ws,
+                  size_t bytes, cudaStream_t st) {
   using raw = typename Elem<DT>::raw;
   const int64_t numel = rows * cols;
-  for (int64_t i = 0; i < batch; i += p.cap) {
-    const int64_t n = batch - i < p.cap ? batch - i : p.cap;
-    NsBatch b;
-    double* partials;
-    carve(&b, p, ws, n, rows, cols, &partials);
+  int64_t cap = int64_t((bytes - kHeader) / matrix_bytes(rows, cols));
+  if (cap > kMaxPass) cap = kMaxPass;
+  for (int64_t i = 0; i < batch; i += cap) {
+    const int64_t n = batch - i < cap ? batch - i : cap;
+    Pass pass(ws);
+    Group& g = pass.add(n, rows, cols, i);
     const raw* x = static_cast<const raw*>(src) + i * numel;
-    const Shape sh{rows, cols, b.ld_x, b.plane_x};
+    const Shape sh{rows, cols, g.b.ld_x, g.b.plane_x};
     int64_t slice = kSliceBytes / (numel * int64_t(sizeof(raw)));
     if (slice < 1) slice = 1;
     for (int64_t k = 0; k < n; k += slice) {
       const unsigned m = unsigned(n - k < slice ? n - k : slice);
-      double* part = partials + k * p.n_partials;
-      square_sum_kernel<DT><<<dim3(unsigned(p.n_partials), m), kThreads, 0, st>>>(
-          x + k * numel, numel, p.chunk, part, i == 0 && k == 0 ? b.error : nullptr);
-      load_kernel<<<dim3(load_grid(b), m), kThreads, 0, st>>>(PlainSource<DT>{x + k * numel, numel}, sh, p.n_partials, part,
-                                                             ns.eps, int(k), b.hi[0], b.lo, b.counter);
+      double* part = g.partials + k * g.n_partials;
+      square_sum_kernel<DT><<<dim3(unsigned(g.n_partials), m), kThreads, 0, st>>>(
+          x + k * numel, numel, g.chunk, part, i == 0 && k == 0 ? g.b.error : nullptr);
+      load_kernel<<<dim3(load_grid(g.b), m), kThreads, 0, st>>>(PlainSource<DT>{x + k * numel, numel}, sh, g.n_partials,
+                                                               part, ns.eps, int(k), g.b.hi[0], g.b.lo, g.b.counter);
     }
     int rc = check_launch("ha_orthogonalize (load)");
-    int at = 0;
-    if (rc == HA_OK) rc = ns_run(b, ns.coef, ns.steps, &at, st);
+    if (rc == HA_OK) rc = pass.run(ns, st);
     if (rc != HA_OK) return rc;
     store_kernel<<<dim3(unsigned((n * numel + kLoadChunk - 1) / kLoadChunk)), kThreads, 0, st>>>(
-        b.hi[at], sh, n * numel, static_cast<uint16_t*>(dst) + i * numel, b.error);
+        g.b.hi[g.b.out], sh, n * numel, static_cast<uint16_t*>(dst) + i * numel, g.b.error);
     rc = check_launch("ha_orthogonalize (store)");
     if (rc != HA_OK) return rc;
   }
@@ -561,47 +572,61 @@ void launch_apply(dim3 grid, cudaStream_t st, const Slice& s, const __half* x, c
 }
 
 template <int DT>
-int muon_step(const ha_tensor* t, int64_t n, int64_t rows, int64_t cols, const MuonConst& c, const ha_ns_params& ns,
-              bool delta, const Peers& peers, unsigned long long* changed, uint32_t* status, const Plan& p, void* ws,
+int muon_step(const ha_tensor* t, const int64_t* shape, int64_t n, const MuonConst& c, const ha_ns_params& ns, bool delta,
+              const Peers& peers, unsigned long long* changed, uint32_t* status, void* ws, size_t bytes,
               cudaStream_t st) {
   int64_t next = 0;  // entries looked at
   bool fresh = true;
   while (next < n) {
-    // the entries of this pass: those with a gradient, as many as the workspace holds
-    const int64_t begin = next;
-    int64_t count = 0;
-    for (; next < n && count < p.cap; ++next) count += t[next].grad != 0;
-    if (count == 0) break;
-    NsBatch b;
-    double* partials;
-    carve(&b, p, ws, count, rows, cols, &partials);
-    const Shape sh{rows, cols, b.ld_x, b.plane_x};
-    int at = 0;
+    // The entries of this pass: those with a gradient, as many as the workspace and a run hold; equal shapes
+    // that follow one another make a group.
+    Pass pass(ws);
+    while (next < n && pass.groups < kNsShapes && (pass.groups + 1) * ns_stages(ns.steps) <= kNsStages) {
+      const int64_t rows = shape[2 * next], cols = shape[2 * next + 1], begin = next;
+      const size_t each = matrix_bytes(rows, cols);
+      int64_t count = 0;
+      bool full = false;
+      for (; next < n && shape[2 * next] == rows && shape[2 * next + 1] == cols; ++next) {
+        if (t[next].grad == 0) continue;
+        full = pass.used + size_t(count + 1) * each > bytes || pass.matrices + count + 1 > kMaxPass;
+        if (full) break;
+        ++count;
+      }
+      if (count > 0) pass.add(count, rows, cols, begin);
+      if (full) break;
+    }
+    if (pass.groups == 0) continue;
     for (int stage = 0; stage < 2; ++stage) {  // momentum and load; then, after the products, the weights
-      MuonSource<DT> src;
-      src.c = c;
-      int64_t k = begin, first = 0;
-      while (first < count) {
-        int m = 0;
-        for (; k < next && m < kSlice; ++k)
-          if (t[k].grad != 0) src.s.t[m++] = t[k];
-        if (stage == 0) {
-          double* part = partials + first * p.n_partials;
-          momentum_kernel<DT><<<dim3(unsigned(p.n_partials), unsigned(m)), kThreads, 0, st>>>(
-              src.s, c, p.chunk, part, fresh ? b.error : nullptr);
-          load_kernel<<<dim3(load_grid(b), unsigned(m)), kThreads, 0, st>>>(src, sh, p.n_partials, part, ns.eps,
-                                                                           int(first), b.hi[0], b.lo,
-                                                                           b.counter);
-          fresh = false;
-        } else {
-          launch_apply<DT>(dim3(unsigned((rows * cols + kApplyChunk - 1) / kApplyChunk), unsigned(m)), st, src.s,
-                           b.hi[at], sh, int(first), c.use_decay, delta, peers, changed, b.error, status);
+      for (int i = 0; i < pass.groups; ++i) {
+        const Group& g = pass.group[i];
+        const int64_t rows = g.b.rows, cols = g.b.cols;
+        const Shape sh{rows, cols, g.b.ld_x, g.b.plane_x};
+        MuonSource<DT> src;
+        src.c = c;
+        // momentum and load of a slice follow one another while it is in L2
+        int64_t slice = kSliceBytes / (rows * cols * (4 + int64_t(sizeof(typename Elem<DT>::raw))));
+        slice = stage != 0 || slice > kSlice ? kSlice : (slice < 1 ? 1 : slice);
+        for (int64_t k = g.begin, first = 0; first < g.b.n;) {
+          int m = 0;
+          for (; m < slice && first + m < g.b.n; ++k)
+            if (t[k].grad != 0) src.s.t[m++] = t[k];
+          if (stage == 0) {
+            double* part = g.partials + first * g.n_partials;
+            momentum_kernel<DT><<<dim3(unsigned(g.n_partials), unsigned(m)), kThreads, 0, st>>>(
+                src.s, c, g.chunk, part, fresh ? g.b.error : nullptr);
+            load_kernel<<<dim3(load_grid(g.b), unsigned(m)), kThreads, 0, st>>>(
+                src, sh, g.n_partials, part, ns.eps, int(first), g.b.hi[0], g.b.lo, g.b.counter);
+            fresh = false;
+          } else {
+            launch_apply<DT>(dim3(unsigned((rows * cols + kApplyChunk - 1) / kApplyChunk), unsigned(m)), st, src.s,
+                             g.b.hi[g.b.out], sh, int(first), c.use_decay, delta, peers, changed, g.b.error, status);
+          }
+          if (int rc = check_launch(stage == 0 ? "ha_muon_step (momentum)" : "ha_muon_step (weights)")) return rc;
+          first += m;
         }
-        if (int rc = check_launch(stage == 0 ? "ha_muon_step (momentum)" : "ha_muon_step (weights)")) return rc;
-        first += m;
       }
       if (stage == 0)
-        if (int rc = ns_run(b, ns.coef, ns.steps, &at, st)) return rc;
+        if (int rc = pass.run(ns, st)) return rc;
     }
   }
   return HA_OK;
@@ -616,7 +641,7 @@ extern "C" int ha_orthogonalize_workspace(int64_t batch, int64_t rows, int64_t c
   if (batch < 0) return fail(HA_ERR_INVALID, "ha_orthogonalize_workspace: batch %lld", (long long)batch);
   if (int rc = check_shape("ha_orthogonalize_workspace", rows, cols)) return rc;
   const int64_t n = batch < 1 ? 1 : (batch > kMaxPass ? kMaxPass : batch);
-  *out = workspace_for(n, rows, cols);
+  *out = kHeader + size_t(n) * matrix_bytes(rows, cols);
   return HA_OK;
 }
 
@@ -633,17 +658,16 @@ extern "C" int ha_orthogonalize(const void* src, int src_dtype, void* dst, int64
   const uintptr_t elem = src_dtype == HA_F32 ? 4 : 2;
   if ((reinterpret_cast<uintptr_t>(src) % elem) != 0 || (reinterpret_cast<uintptr_t>(dst) & 1) != 0)
     return fail(HA_ERR_INVALID, "ha_orthogonalize: misaligned matrices");
-  Plan p;
-  if (int rc = make_plan("ha_orthogonalize", batch, rows, cols, workspace, workspace_bytes, &p)) return rc;
+  if (int rc = check_workspace("ha_orthogonalize", rows, cols, workspace, workspace_bytes)) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   switch (src_dtype) {
-    case HA_F32: return orthogonalize<HA_F32>(src, dst, batch, rows, cols, *ns, p, workspace, st);
-    case HA_BF16: return orthogonalize<HA_BF16>(src, dst, batch, rows, cols, *ns, p, workspace, st);
-    default: return orthogonalize<HA_F16>(src, dst, batch, rows, cols, *ns, p, workspace, st);
+    case HA_F32: return orthogonalize<HA_F32>(src, dst, batch, rows, cols, *ns, workspace, workspace_bytes, st);
+    case HA_BF16: return orthogonalize<HA_BF16>(src, dst, batch, rows, cols, *ns, workspace, workspace_bytes, st);
+    default: return orthogonalize<HA_F16>(src, dst, batch, rows, cols, *ns, workspace, workspace_bytes, st);
   }
 }
 
-extern "C" int ha_muon_step(const ha_tensor* h_tensors, int64_t n, int64_t rows, int64_t cols, int grad_dtype,
+extern "C" int ha_muon_step(const ha_tensor* h_tensors, const int64_t* h_shapes, int64_t n, int grad_dtype,
                             const ha_muon_scalars* sc, const ha_ns_params* ns, int changed_only, const ha_peers* peers,
                             unsigned long long* d_changed_groups, uint32_t* d_status, void* workspace,
                             size_t workspace_bytes, void* stream) {
@@ -652,7 +676,6 @@ extern "C" int ha_muon_step(const ha_tensor* h_tensors, int64_t n, int64_t rows,
   if (!valid_float_dtype(grad_dtype)) return fail(HA_ERR_UNSUPPORTED, "ha_muon_step: grad dtype %d", grad_dtype);
   if (n < 0) return fail(HA_ERR_INVALID, "ha_muon_step: %lld tensors", (long long)n);
   if (sc == nullptr) return fail(HA_ERR_INVALID, "ha_muon_step: NULL scalars");
-  if (int rc = check_shape("ha_muon_step", rows, cols)) return rc;
   if (int rc = check_steps("ha_muon_step", ns)) return rc;
   Peers q{};
   if (peers != nullptr) {
@@ -665,28 +688,32 @@ extern "C" int ha_muon_step(const ha_tensor* h_tensors, int64_t n, int64_t rows,
     }
   }
   if (n == 0) return HA_OK;
-  if (h_tensors == nullptr) return fail(HA_ERR_INVALID, "ha_muon_step: NULL table");
+  if (h_tensors == nullptr || h_shapes == nullptr) return fail(HA_ERR_INVALID, "ha_muon_step: NULL table");
   const uint64_t elem = grad_dtype == HA_F32 ? 3 : 1;
   for (int64_t i = 0; i < n; ++i) {
     const ha_tensor& t = h_tensors[i];
+    const int64_t rows = h_shapes[2 * i], cols = h_shapes[2 * i + 1];
+    if (int rc = check_shape("ha_muon_step", rows, cols)) return rc;
     if (t.grad == 0) continue;
     if (t.numel != rows * cols || t.master == 0 || t.exp_avg == 0 || (grad_dtype != HA_F32 && t.param == 0))
       return fail(HA_ERR_INVALID, "ha_muon_step: entry %lld: %lld elements for %lld x %lld, or a NULL address",
                   (long long)i, (long long)t.numel, (long long)rows, (long long)cols);
     if (((t.grad | t.param) & elem) != 0 || ((t.master | t.exp_avg) & 3) != 0)
       return fail(HA_ERR_INVALID, "ha_muon_step: entry %lld: misaligned address", (long long)i);
+    if (int rc = check_workspace("ha_muon_step", rows, cols, workspace, workspace_bytes)) return rc;
   }
-  Plan p;
-  if (int rc = make_plan("ha_muon_step", n, rows, cols, workspace, workspace_bytes, &p)) return rc;
   const MuonConst c{sc->mu, sc->one_minus_mu, sc->nesterov, sc->use_decay, sc->clip, sc->clip_mult};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool delta = changed_only != 0 && grad_dtype != HA_F32;
   switch (grad_dtype) {
     case HA_F32:
-      return muon_step<HA_F32>(h_tensors, n, rows, cols, c, *ns, delta, q, d_changed_groups, d_status, p, workspace, st);
+      return muon_step<HA_F32>(h_tensors, h_shapes, n, c, *ns, delta, q, d_changed_groups, d_status, workspace,
+                               workspace_bytes, st);
     case HA_BF16:
-      return muon_step<HA_BF16>(h_tensors, n, rows, cols, c, *ns, delta, q, d_changed_groups, d_status, p, workspace, st);
+      return muon_step<HA_BF16>(h_tensors, h_shapes, n, c, *ns, delta, q, d_changed_groups, d_status, workspace,
+                               workspace_bytes, st);
     default:
-      return muon_step<HA_F16>(h_tensors, n, rows, cols, c, *ns, delta, q, d_changed_groups, d_status, p, workspace, st);
+      return muon_step<HA_F16>(h_tensors, h_shapes, n, c, *ns, delta, q, d_changed_groups, d_status, workspace,
+                               workspace_bytes, st);
   }
 }

@@ -21,12 +21,15 @@
 // replaces two products with X (6 m^2 n of 2 (3 m^2 n + m^3)) by one and three more symmetric ones:
 // 3 m^2 n + 5 m^3.  See pairs() for where that is done and what it costs in accuracy.
 //
-// All products of all steps run in one persistent launch, one CTA per SM, one or two CTAs to a tile:
-// a step of a small matrix takes a few microseconds, less than what three launches cost.  The work is a list
-// of stages (one product of every matrix of the batch each), whose tiles the CTAs take in turn; a tile of
-// a stage waits until all tiles of the previous stage of the same matrix are stored (a counter per matrix in
-// global memory), so the matrices of a batch need not wait for one another and a stage's last tiles run beside
-// the next one's first.  The launch is cooperative: all CTAs are resident, so the waits end.
+// All products of all steps of all shapes run in one persistent launch, one CTA per SM, one or two CTAs to a
+// tile: a step of a small matrix takes a few microseconds, less than what three launches cost.  The work is a list
+// of jobs (a stage, that is one product, of some matrices of one shape), whose tiles the CTAs take in turn; a tile
+// waits until all tiles of the previous stage of its matrix are stored (a counter per matrix in global memory), so
+// matrices need not wait for one another and a job's last tiles run beside the next one's first.  Jobs of several
+// shapes alternate, so that one shape's tiles fill the time in which another's results travel; of a batch that
+// does not fit L2, X is multiplied a few matrices at a time, each followed soon by its Gram matrix, which then finds
+// X in L2 and gives the tensor cores work while the next X streams through.  A job waits only for jobs before it
+// in the list, and the launch is cooperative: all CTAs are resident, so the waits end.
 //
 // In a CTA, warp 0 feeds a ring of 128-byte-swizzled operand tiles by TMA, one thread of warp 1 issues the
 // MMAs, and eight epilogue warps read the accumulators from one of two TMEM buffers while the next tile
@@ -38,6 +41,7 @@
 // transposed: both operand layouts (K contiguous, or M/N contiguous) are read by the MMA as they lie.
 #include <cuda.h>
 
+#include <algorithm>
 #include <cmath>
 
 #include "ha_common.cuh"
@@ -51,6 +55,7 @@ constexpr int kBM = 128;           // rows of a CTA's part of a tile: the TMEM l
 constexpr int kBK = 64;            // K elements of a ring slot: one 128-byte swizzle row
 constexpr int kGemmThreads = 416;  // operands, MMA, addends, stores; eight epilogue warps; stores
 constexpr int kPreciseSteps = 3;
+constexpr int64_t kCacheBytes = 64 << 20;  // planes that stay in L2 (126 MB) beside the rest of a stage
 constexpr int kHalf = kBM * kBK * 2;  // bytes of one operand's part of a slot
 constexpr int kSlot = 2 * kHalf;
 constexpr int kSlots = 5;
@@ -80,22 +85,33 @@ enum Map {
 
 struct Stage {
   int M, N, K;        // D is M x N
-  int tiles_m, tiles_n, per_matrix, tiles;
-  int skew;           // tiles of the stages before, modulo the CTAs (or pairs): the list goes on where it stopped
+  int tiles_m, tiles_n, per_matrix;
   uint32_t before;    // a matrix's counter when its previous stage is stored
-  int8_t epilogue, m_fast, a_mn, b_mn;  // *_mn: the operand's M / N index is the contiguous one
-  int8_t map_a, map_b, map_out, map_2, map_add, keep_low;
+  int counter;        // of the shape's first matrix
   float scale, add, diag;
+  uint8_t map_a, map_b, map_out, map_2, map_add;
+  int8_t epilogue, m_fast, a_mn, b_mn, keep_low;  // *_mn: the operand's M / N index is the contiguous one
 };
-constexpr int kMaxStages = 3 * HA_NS_MAX_STEPS + 2;
+// A stage of `count` matrices from `first` on.
+struct Job {
+  uint16_t stage, first, count, reserved;
+};
 
-struct RunArgs {
-  CUtensorMap map[kMaps];
-  Stage stage[kMaxStages];
-  int stages;
+// Kernel parameters; small ones launch faster.
+template <int SHAPES, int STAGES, int JOBS>
+struct RunArgsOf {
+  CUtensorMap map[SHAPES * kMaps];
+  Stage stage[STAGES];
+  Job job[JOBS];
+  int jobs;
   uint32_t* counter;  // one for each matrix
   uint32_t* error;
 };
+constexpr int kMaxStages = 3 * HA_NS_MAX_STEPS + 2;  // of one shape
+constexpr int kManyShapes = kNsShapes, kManyStages = kNsStages, kManyJobs = 1024;
+using OneShape = RunArgsOf<1, kMaxStages, kMaxStages>;
+using ManyShapes = RunArgsOf<kManyShapes, kManyStages, kManyJobs>;
+static_assert(sizeof(ManyShapes) <= 32000, "kernel parameters");
 
 __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
@@ -108,11 +124,12 @@ __device__ __forceinline__ float2 unpack_half2(uint32_t w) {
 struct TileAt {
   int z, i, j;  // matrix, tile row, tile column
 };
-// Symmetric stages: the tiles on and below the diagonal, row by row.
-__device__ __forceinline__ TileAt tile_at(const Stage& g, int t) {
+// Tile `t` of a job.  Symmetric stages: the tiles on and below the diagonal, row by row.
+__device__ __forceinline__ TileAt tile_at(const Stage& g, const Job& job, int t) {
   TileAt a;
   a.z = t / g.per_matrix;
   const int r = t - a.z * g.per_matrix;
+  a.z += job.first;
   if (g.epilogue <= kPoly) {
     int i = int((sqrtf(8.0f * float(r) + 1.0f) - 1.0f) * 0.5f);
     while (i * (i + 1) / 2 > r) --i;
@@ -128,10 +145,13 @@ __device__ __forceinline__ TileAt tile_at(const Stage& g, int t) {
   }
   return a;
 }
-__device__ __forceinline__ int first_tile(const Stage& g, int first, int step) {
-  const int t = first - g.skew;
-  return t < 0 ? t + step : t;
-}
+// A CTA's (or pair's) walk through the jobs: tiles `first`, `first` + `step`, .. of the whole list.
+struct Walk {
+  int first, step;
+  int skew = 0;  // tiles of the jobs before, modulo `step`
+  __device__ __forceinline__ int start() const { return first >= skew ? first - skew : first - skew + step; }
+  __device__ __forceinline__ void pass(int tiles) { skew = (skew + tiles) % step; }
+};
 
 // Blocks of a CTA's part of a tile: those that reach into D.
 template <int CG>
@@ -152,7 +172,8 @@ struct Shared {
 
 // One of the eight epilogue warps, kept over all stages.
 struct Warp {
-  int lane, quarter, group, step, first, rank;
+  int lane, quarter, group, rank;
+  Walk walk;
   uint32_t ring;           // shared memory: blocks, then their second results
   uint32_t tmem;           // its lanes of the accumulators
   uint32_t n;              // blocks of this CTA so far
@@ -160,7 +181,7 @@ struct Warp {
 };
 
 template <int CG, int EPI>
-__device__ __forceinline__ bool epilogue(const Stage& g, Warp& w, Shared& sh) {
+__device__ __forceinline__ bool epilogue(const Stage& g, const Job& job, Warp& w, Shared& sh) {
   constexpr bool kSym = EPI == kSymmetric || EPI == kPoly;
   constexpr bool kAdd = EPI == kPoly || EPI == kPrecise;
   constexpr int kTile = 128 * CG;
@@ -168,8 +189,9 @@ __device__ __forceinline__ bool epilogue(const Stage& g, Warp& w, Shared& sh) {
   const int mine = w.quarter * 32 + lane;                            // this lane's row of a block:
   const uint32_t row_at = mine * 64, key = (uint32_t(mine) >> 1) & 3;  // its 16-byte piece j lies at j ^ key
   const float scale = g.scale, add_scale = g.add, diag = g.diag;
-  for (int t = first_tile(g, w.first, w.step); t < g.tiles; t += w.step) {
-    const TileAt at = tile_at(g, t);
+  const int tiles = job.count * g.per_matrix;
+  for (int t = w.walk.start(); t < tiles; t += w.walk.step) {
+    const TileAt at = tile_at(g, job, t);
     const int blocks = blocks_of<CG>(g, at, w.rank);
     const int row = at.i * kTile + w.rank * kBM + mine;
     if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&sh.acc_full[w.acc]), w.acc_phase, &sh.stop))) return false;
@@ -256,15 +278,17 @@ __device__ __forceinline__ bool epilogue(const Stage& g, Warp& w, Shared& sh) {
 }
 
 // Warp 2, one thread: a block's addend, or only the block itself, to the epilogue warps.
-template <int CG>
-__device__ __forceinline__ void feed_blocks(const RunArgs& p, Shared& sh, uint32_t ring, int first, int step, int rank) {
+template <int CG, class Args>
+__device__ __forceinline__ void feed_blocks(const Args& p, Shared& sh, uint32_t ring, Walk walk, int rank) {
   uint32_t n = 0, tile = 0;
-  for (int s = 0; s < p.stages; ++s) {
-    const Stage& g = p.stage[s];
+  for (int q = 0; q < p.jobs; ++q) {
+    const Job job = p.job[q];
+    const Stage& g = p.stage[job.stage];
     const bool add = g.epilogue == kPoly || g.epilogue == kPrecise;
-    for (int t = first_tile(g, first, step); t < g.tiles; t += step) {
+    const int tiles = job.count * g.per_matrix;
+    for (int t = walk.start(); t < tiles; t += walk.step) {
       ++tile;
-      const TileAt at = tile_at(g, t);
+      const TileAt at = tile_at(g, job, t);
       const int blocks = blocks_of<CG>(g, at, rank);
       for (int k = 0; k < blocks; ++k, ++n) {
         const uint32_t b = n % kBlocks, full = smem_u32(&sh.blk_full[b]);
@@ -279,18 +303,22 @@ __device__ __forceinline__ void feed_blocks(const RunArgs& p, Shared& sh, uint32
                        at.i * (128 * CG) + rank * kBM, at.z);
       }
     }
+    walk.pass(tiles);
   }
 }
 
 // Warps 3 and 12, one thread each: the blocks that one epilogue group finished, to memory; then the counter.
-template <int CG>
-__device__ __forceinline__ void store_blocks(const RunArgs& p, Shared& sh, uint32_t ring, int first, int step, int rank,
+template <int CG, class Args>
+__device__ __forceinline__ void store_blocks(const Args& p, Shared& sh, uint32_t ring, Walk walk, int rank,
                                              uint32_t group) {
-  uint32_t n = 0;
-  for (int s = 0; s < p.stages; ++s) {
-    const Stage& g = p.stage[s];
-    for (int t = first_tile(g, first, step); t < g.tiles; t += step) {
-      const TileAt at = tile_at(g, t);
+  uint32_t n = 0, tile = 0;
+  for (int q = 0; q < p.jobs; ++q) {
+    const Job job = p.job[q];
+    const Stage& g = p.stage[job.stage];
+    const int tiles = job.count * g.per_matrix;
+    for (int t = walk.start(); t < tiles; t += walk.step) {
+      ++tile;
+      const TileAt at = tile_at(g, job, t);
       const int blocks = blocks_of<CG>(g, at, rank), row = at.i * (128 * CG) + rank * kBM;
       uint32_t last = kBlocks;  // block of the store before, not yet handed back
       for (int k = int((n ^ group) & 1); k < blocks; k += 2) {
@@ -313,16 +341,22 @@ __device__ __forceinline__ void store_blocks(const RunArgs& p, Shared& sh, uint3
       }
       n += blocks;
       tma_store_wait_all();
-      if (last < kBlocks) mbar_arrive(smem_u32(&sh.blk_free[last]));
-      counter_raise(p.counter + at.z);
+      // A tile without blocks of this group must not be counted before its matrix's previous stage is stored:
+      // the counter tells stages apart only as long as they are raised one after another.
+      if (last < kBlocks)
+        mbar_arrive(smem_u32(&sh.blk_free[last]));
+      else if (!granted_wait(&sh.granted, tile, &sh.stop))
+        return;
+      counter_raise(p.counter + g.counter + at.z);
     }
+    walk.pass(tiles);
   }
 }
 
 // CG: CTAs of a tile (1: 128 x 128; 2: 256 x 256, each CTA with 128 rows of A and of D and 128 columns
 // of B).
-template <int CG>
-__global__ void __launch_bounds__(kGemmThreads, 1) newton_schulz_kernel(const __grid_constant__ RunArgs p) {
+template <int CG, class Args>
+__global__ void __launch_bounds__(kGemmThreads, 1) newton_schulz_kernel(const __grid_constant__ Args p) {
   constexpr int kTile = 128 * CG;         // rows and columns of a tile
   constexpr int kColumns = 2 * kTile;     // TMEM columns: two accumulators
   extern __shared__ uint8_t smem_raw[];
@@ -350,7 +384,6 @@ __global__ void __launch_bounds__(kGemmThreads, 1) newton_schulz_kernel(const __
     }
     mbar_fence_init();
   }
-  if (warp == 0 && lane < kMaps) tma_prefetch_map(&p.map[lane]);
   if (warp == 1) tmem_alloc<CG>(smem_u32(&sh.tmem), kColumns);
   tc_fence_before();
   if (CG == 2)
@@ -359,23 +392,25 @@ __global__ void __launch_bounds__(kGemmThreads, 1) newton_schulz_kernel(const __
     __syncthreads();
   tc_fence_after();
   const uint32_t tmem = sh.tmem;
-  const int first = blockIdx.x / CG, step = gridDim.x / CG;
+  Walk walk{int(blockIdx.x) / CG, int(gridDim.x) / CG};
 
   if (warp == 0) {
     if (elect_one()) {
       int slot = 0;
       uint32_t phase = 0, tile = 0;
       bool ok = true;
-      for (int s = 0; s < p.stages && ok; ++s) {
-        const Stage& g = p.stage[s];
+      for (int q = 0; q < p.jobs && ok; ++q) {
+        const Job job = p.job[q];
+        const Stage& g = p.stage[job.stage];
+        const int tiles = job.count * g.per_matrix;
         const CUtensorMap *map_a = &p.map[g.map_a], *map_b = &p.map[g.map_b];
         const int kblocks = (g.K + kBK - 1) / kBK;
         const bool a_mn = g.a_mn, b_mn = g.b_mn;
         int ready = -1;
-        for (int t = first_tile(g, first, step); t < g.tiles && ok; t += step) {
-          const TileAt at = tile_at(g, t);
+        for (int t = walk.start(); t < tiles && ok; t += walk.step) {
+          const TileAt at = tile_at(g, job, t);
           if (at.z != ready) {
-            ok = counter_wait(p.counter + at.z, g.before, &sh.stop);
+            ok = counter_wait(p.counter + g.counter + at.z, g.before, &sh.stop);
             if (!ok) break;
             ready = at.z;
           }
@@ -403,6 +438,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) newton_schulz_kernel(const __
             if (++slot == kSlots) slot = 0, phase ^= 1;
           }
         }
+        walk.pass(tiles);
       }
     }
     __syncwarp();
@@ -411,13 +447,15 @@ __global__ void __launch_bounds__(kGemmThreads, 1) newton_schulz_kernel(const __
       int slot = 0;
       uint32_t phase = 0, acc = 0, acc_phase = 0;
       bool ok = true;
-      for (int s = 0; s < p.stages && ok; ++s) {
-        const Stage& g = p.stage[s];
+      for (int q = 0; q < p.jobs && ok; ++q) {
+        const Job job = p.job[q];
+        const Stage& g = p.stage[job.stage];
+        const int tiles = job.count * g.per_matrix;
         const int kblocks = (g.K + kBK - 1) / kBK;
         const uint32_t idesc = f16_idesc(kTile, kTile, g.a_mn, g.b_mn);
         const uint32_t lead_a = g.a_mn ? 8192 : 16, lead_b = g.b_mn ? 8192 : 16;
         const uint32_t next_a = g.a_mn ? kStepMN : kStepK, next_b = g.b_mn ? kStepMN : kStepK;
-        for (int t = first_tile(g, first, step); t < g.tiles && ok; t += step) {
+        for (int t = walk.start(); t < tiles && ok; t += walk.step) {
           ok = mbar_wait(smem_u32(&sh.acc_empty[acc]), acc_phase ^ 1, &sh.stop);
           if (!ok) break;
           tc_fence_after();
@@ -437,15 +475,16 @@ __global__ void __launch_bounds__(kGemmThreads, 1) newton_schulz_kernel(const __
           if (ok) mma_commit<CG>(smem_u32(&sh.acc_full[acc]));
           if (++acc == 2) acc = 0, acc_phase ^= 1;
         }
+        walk.pass(tiles);
       }
     }
     __syncwarp();
   } else if (warp == 2) {
-    if (lane == 0) feed_blocks<CG>(p, sh, ring + kSlots * kSlot, first, step, int(rank));
+    if (lane == 0) feed_blocks<CG>(p, sh, ring + kSlots * kSlot, walk, int(rank));
     __syncwarp();
   } else if (warp == 3 || warp == 12) {
     if (lane == 0) {
-      store_blocks<CG>(p, sh, ring + kSlots * kSlot, first, step, int(rank), warp == 3 ? 0 : 1);
+      store_blocks<CG>(p, sh, ring + kSlots * kSlot, walk, int(rank), warp == 3 ? 0 : 1);
       tma_store_wait_all();
     }
     __syncwarp();
@@ -454,20 +493,21 @@ __global__ void __launch_bounds__(kGemmThreads, 1) newton_schulz_kernel(const __
     w.lane = lane;
     w.quarter = warp & 3;  // the TMEM lanes this warp may read: 32 * quarter ..
     w.group = (warp - 4) >> 2;
-    w.step = step;
-    w.first = first;
+    w.walk = walk;
     w.rank = int(rank);
     w.ring = ring + kSlots * kSlot;
     w.tmem = tmem + (uint32_t(w.quarter * 32) << 16);
     bool ok = true;
-    for (int s = 0; s < p.stages && ok; ++s) {
-      const Stage& g = p.stage[s];
+    for (int q = 0; q < p.jobs && ok; ++q) {
+      const Job job = p.job[q];
+      const Stage& g = p.stage[job.stage];
       switch (g.epilogue) {
-        case kSymmetric: ok = epilogue<CG, kSymmetric>(g, w, sh); break;
-        case kPoly: ok = epilogue<CG, kPoly>(g, w, sh); break;
-        case kPrecise: ok = epilogue<CG, kPrecise>(g, w, sh); break;
-        default: ok = epilogue<CG, kPlain>(g, w, sh); break;
+        case kSymmetric: ok = epilogue<CG, kSymmetric>(g, job, w, sh); break;
+        case kPoly: ok = epilogue<CG, kPoly>(g, job, w, sh); break;
+        case kPrecise: ok = epilogue<CG, kPrecise>(g, job, w, sh); break;
+        default: ok = epilogue<CG, kPlain>(g, job, w, sh); break;
       }
+      w.walk.pass(job.count * g.per_matrix);
     }
   }
   __syncthreads();
@@ -550,10 +590,10 @@ int pairs(int64_t m, int64_t n, const float* coef, int steps) {
   return count;
 }
 
-int make_maps(const NsBatch& b, RunArgs* p) {
+int make_maps(const NsBatch& b, CUtensorMap* maps) {
   int rc = HA_OK;
   auto map = [&](int to, const Operand& x, int cols, int rows, CUtensorMapSwizzle swizzle) {
-    if (rc == HA_OK) rc = make_map(&p->map[to], x, b.n, cols, rows, swizzle);
+    if (rc == HA_OK) rc = make_map(&maps[to], x, b.n, cols, rows, swizzle);
   };
   auto operand = [&](int to, const Operand& x, int rows) { map(to, x, 64, rows, CU_TENSOR_MAP_SWIZZLE_128B); };
   auto block = [&](int to, const Operand& x) { map(to, x, kBlockCols, kBM, CU_TENSOR_MAP_SWIZZLE_64B); };
@@ -573,14 +613,16 @@ int make_maps(const NsBatch& b, RunArgs* p) {
   return rc;
 }
 
-// The stages of a run; returns the index of the plane with the result.
-int make_stages(const NsBatch& b, const float* coef, int steps, RunArgs* p) {
+// The stages of a shape, whose maps start at `map0` and counters at `counter`; returns their number.
+int make_stages(NsBatch* shape, const float* coef, int steps, int map0, int counter, Stage* stages) {
+  const NsBatch& b = *shape;
+  int count = 0;
   const bool tall = b.rows > b.cols;
   const int m = int(b.m), n = int(tall ? b.rows : b.cols);
-  p->stages = 0;
   auto add = [&](Epilogue e, int M, int N, int K) {
-    Stage& g = p->stage[p->stages++];
+    Stage& g = stages[count++];
     g = Stage{};
+    g.counter = counter;
     g.epilogue = int8_t(e);
     g.M = M, g.N = N, g.K = K;
     return &g;
@@ -588,11 +630,11 @@ int make_stages(const NsBatch& b, const float* coef, int steps, RunArgs* p) {
   // a symmetric m x m product of square matrices x and y, which commute
   auto multiply = [&](Epilogue e, int x, int y, int to) {
     Stage* g = add(e, m, m, m);
-    g->map_a = int8_t(kMapSq + x);
-    g->map_b = int8_t(kMapSq + y);
-    g->map_out = int8_t(kMapSqOut + to);
-    g->map_2 = int8_t(kMapSqMirror + to);
-    g->map_add = int8_t(kMapSqOut + x);
+    g->map_a = uint8_t(map0 + kMapSq + x);
+    g->map_b = uint8_t(map0 + kMapSq + y);
+    g->map_out = uint8_t(map0 + kMapSqOut + to);
+    g->map_2 = uint8_t(map0 + kMapSqMirror + to);
+    g->map_add = uint8_t(map0 + kMapSqOut + x);
     g->scale = 1.0f / kScaleG;
     return g;
   };
@@ -609,9 +651,9 @@ int make_stages(const NsBatch& b, const float* coef, int steps, RunArgs* p) {
     const float* c = coef + 3 * s;
     Stage* g = add(kSymmetric, m, m, n);
     g->a_mn = g->b_mn = tall;
-    g->map_a = g->map_b = int8_t((tall ? kMapXmn : kMapXk) + cur);
-    g->map_out = kMapSqOut;
-    g->map_2 = kMapSqMirror;
+    g->map_a = g->map_b = uint8_t(map0 + (tall ? kMapXmn : kMapXk) + cur);
+    g->map_out = uint8_t(map0 + kMapSqOut);
+    g->map_2 = uint8_t(map0 + kMapSqMirror);
     g->scale = kScaleG / (kScaleX * kScaleX);
     factor(0, 1, c);
     if (pair) {
@@ -623,46 +665,81 @@ int make_stages(const NsBatch& b, const float* coef, int steps, RunArgs* p) {
     const int q = pair ? 0 : 1;
     g = add(s < kPreciseSteps ? kPrecise : kPlain, int(b.rows), int(b.cols), m);
     g->b_mn = !tall;
-    g->map_a = int8_t(tall ? kMapXk + cur : kMapSq + q);
-    g->map_b = int8_t(tall ? kMapSq + q : kMapXmn + cur);
+    g->map_a = uint8_t(map0 + (tall ? kMapXk + cur : kMapSq + q));
+    g->map_b = uint8_t(map0 + (tall ? kMapSq + q : kMapXmn + cur));
     cur ^= 1;
-    g->map_out = int8_t(kMapXout + cur);
-    g->map_2 = g->map_add = kMapLow;  // rewritten in place, block by block
+    g->map_out = uint8_t(map0 + kMapXout + cur);
+    g->map_2 = g->map_add = uint8_t(map0 + kMapLow);  // rewritten in place, block by block
     g->scale = 1.0f / kScaleG;
     g->add = (pair ? c[0] * c[3] : c[0]) / kScaleLo;
     s += pair ? 2 : 1;
     g->keep_low = s < kPreciseSteps && s < steps;  // the next step reads it
   }
-  return cur;
+  shape->out = cur;
+  return count;
 }
 
-// Cuts the stages into tiles and returns the work of the busiest CTA, in 128 x 128 x 64 products, or -1
-// if there are too many tiles.
-int64_t cut(RunArgs* p, int64_t batch, int cg, int sms) {
-  const int tile = 128 * cg, workers = sms / cg;
-  int64_t skew = 0, cost = 0;
+// Cuts a shape's stages into tiles; adds its work, in 128 x 128 x 64 products of a CTA, to *work, and the
+// work of the busiest CTA, if the shape ran alone, to *alone.  False if there are too many tiles.
+bool cut(Stage* stages, int count, int64_t batch, int cg, int workers, double* work, double* alone) {
+  const int tile = 128 * cg;
   uint32_t before = 0;
-  for (int s = 0; s < p->stages; ++s) {
-    Stage& g = p->stage[s];
+  for (int s = 0; s < count; ++s) {
+    Stage& g = stages[s];
     g.tiles_m = (g.M + tile - 1) / tile;
     g.tiles_n = (g.N + tile - 1) / tile;
     const int64_t per = g.epilogue <= kPoly ? int64_t(g.tiles_m) * (g.tiles_m + 1) / 2 : int64_t(g.tiles_m) * g.tiles_n;
-    if (per * batch > 0x3fffffff || before > 0x7fffffff) return -1;
+    if (per * batch > 0x3fffffff || before > 0x7fffffff) return false;
     g.per_matrix = int(per);
-    g.tiles = int(per * batch);
     g.m_fast = g.tiles_m <= g.tiles_n;  // the shorter side first: its operand panels stay in L2
-    g.skew = int(skew);
     g.before = before;
-    before += uint32_t(per) * 2 * cg;  // both store warps of each of its CTAs
-    skew = (skew + g.tiles) % workers;
-    cost += (g.tiles + workers - 1) / workers * cg * ((g.K + kBK - 1) / kBK);
+    before += uint32_t(per) * 2 * cg;   // both store warps of each of its CTAs
+    const double each = double(cg) * ((g.K + kBK - 1) / kBK);
+    *work += each * double(per * batch) / workers;
+    *alone += each * double((per * batch + workers - 1) / workers);
   }
-  return cost;
+  return true;
 }
 
-template <int CG>
-int launch(const RunArgs& p, int sms, cudaStream_t st) {
-  auto* kernel = newton_schulz_kernel<CG>;
+// The jobs of one shape in the order in which they run, each with the share of the shape's work before it.
+struct Placed {
+  Job job;
+  double at;
+};
+int place(const Stage* stages, int first_stage, int count, const NsBatch& b, int workers, Placed* out, int room) {
+  int n = 0;
+  double total = 0.0, done = 0.0;
+  auto cost = [&](int s) { return double(stages[s].per_matrix) * ((stages[s].K + kBK - 1) / kBK); };
+  for (int s = 0; s < count; ++s) total += cost(s) * double(b.n);
+  auto put = [&](int s, int64_t first, int64_t matrices) {
+    out[n++] = Placed{Job{uint16_t(first_stage + s), uint16_t(first), uint16_t(matrices), 0}, done / total};
+    done += cost(s) * double(matrices);
+  };
+  for (int s = 0; s < count; ++s) {
+    // a product with X and the Gram matrix of its result, a few matrices at a time if the planes exceed L2
+    const bool x = stages[s].epilogue >= kPrecise;
+    int64_t chunk = b.n;
+    if (x && s + 1 < count && b.n * b.plane_x * 6 > kCacheBytes) {
+      chunk = (2 * workers + stages[s].per_matrix - 1) / stages[s].per_matrix;
+      if (chunk * 64 < b.n) chunk = (b.n + 63) / 64;
+    }
+    const int64_t chunks = (b.n + chunk - 1) / chunk;
+    if (chunks < 3 || n + 2 * chunks + (count - s) > room) {
+      put(s, 0, b.n);
+      continue;
+    }
+    for (int64_t c = 0; c <= chunks; ++c) {  // the Gram matrices one chunk behind
+      if (c < chunks) put(s, c * chunk, c * chunk + chunk < b.n ? chunk : b.n - c * chunk);
+      if (c > 0) put(s + 1, (c - 1) * chunk, c < chunks ? chunk : b.n - (c - 1) * chunk);
+    }
+    ++s;
+  }
+  return n;
+}
+
+template <int CG, class Args>
+int launch(const Args& p, int sms, cudaStream_t st) {
+  auto* kernel = newton_schulz_kernel<CG, Args>;
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kGemmSmem) != cudaSuccess)
     return check_launch("newton_schulz_kernel (shared memory)");
   cudaLaunchConfig_t cfg{};
@@ -685,6 +762,45 @@ int launch(const RunArgs& p, int sms, cudaStream_t st) {
     return fail(HA_ERR_CUDA, "newton_schulz_kernel: %s", cudaGetErrorString(e));
   }
   return HA_OK;
+}
+
+// One launch for `n` shapes.  The tile: 256 x 256 on a CTA pair reads half the operand bytes per product of a
+// 128 x 128 tile on one CTA and runs 1.35 times as fast where both fill the chip (2.75 against 3.70 ms for five
+// steps of 4096 x 12288), but leaves SMs idle when there are few tiles and pads more.
+template <class Args>
+int run(NsBatch** shapes, int n, const float* coef, int steps, int sms, cudaStream_t st) {
+  constexpr int kRoom = int(sizeof(Args::job) / sizeof(Job));
+  static thread_local Args p;
+  static thread_local Placed list[kRoom];
+  int first[kManyShapes + 1] = {0};
+  for (int i = 0; i < n; ++i) {
+    if (int rc = make_maps(*shapes[i], p.map + i * kMaps)) return rc;
+    first[i + 1] = first[i] + make_stages(shapes[i], coef, steps, i * kMaps, int(shapes[i]->counter - shapes[0]->counter),
+                                          p.stage + first[i]);
+  }
+  auto cost = [&](int cg) {
+    double work = 0.0, longest = 0.0;
+    for (int i = 0; i < n; ++i) {
+      double alone = 0.0;
+      if (!cut(p.stage + first[i], first[i + 1] - first[i], shapes[i]->n, cg, sms / cg, &work, &alone)) return -1.0;
+      if (alone > longest) longest = alone;
+    }
+    return work > longest ? work : longest;
+  };
+  const double two = cost(2), one = cost(1);
+  if (one < 0) return fail(HA_ERR_INVALID, "Newton-Schulz products with too many tiles");
+  const int cg = 1.35 * one <= two ? 1 : 2;
+  if (cg == 2) cost(2);
+  int jobs = 0;
+  for (int i = 0; i < n; ++i)
+    jobs += place(p.stage + first[i], first[i], first[i + 1] - first[i], *shapes[i], sms / cg, list + jobs,
+                  (kRoom - jobs) / (n - i));
+  std::stable_sort(list, list + jobs, [](const Placed& a, const Placed& b) { return a.at < b.at; });
+  for (int q = 0; q < jobs; ++q) p.job[q] = list[q].job;
+  p.jobs = jobs;
+  p.counter = shapes[0]->counter;
+  p.error = shapes[0]->error;
+  return cg == 1 ? launch<1>(p, sms, st) : launch<2>(p, sms, st);
 }
 
 int64_t up(int64_t x, int64_t a) { return (x + a - 1) / a * a; }
@@ -741,23 +857,23 @@ void ns_carve(NsBatch* b, void* base) {
   for (int i = 0; i < 3; ++i) b->square[i] = b->lo + b->n * b->plane_x + i * b->n * b->plane_g;
 }
 
-int ns_run(const NsBatch& b, const float* coef, int steps, int* out, cudaStream_t st) {
+int ns_stages(int steps) { return 3 * steps + 2; }
+
+int ns_run(NsBatch* shapes, int n, const float* coef, int steps, cudaStream_t st) {
   int sms = 0;
   if (int rc = sm_count(&sms)) return rc;
-  if (narrow_fits(b.rows, b.cols, coef, steps)) return narrow_run(b, coef, steps, out, sms, st);
-  RunArgs p;
-  if (int rc = make_maps(b, &p)) return rc;
-  p.counter = b.counter;
-  p.error = b.error;
-  *out = make_stages(b, coef, steps, &p);
-  // The tile: 256 x 256 on a CTA pair reads half the operand bytes per product of a 128 x 128 tile on one
-  // CTA and runs 1.35 times as fast where both fill the chip (2.75 against 3.70 ms for five steps of
-  // 4096 x 12288), but leaves SMs idle when there are few tiles and pads more.
-  const int64_t two = cut(&p, b.n, 2, sms), one = cut(&p, b.n, 1, sms);
-  if (one < 0) return fail(HA_ERR_INVALID, "Newton-Schulz products with too many tiles");
-  if (1.35 * double(one) <= double(two)) return launch<1>(p, sms, st);
-  cut(&p, b.n, 2, sms);
-  return launch<2>(p, sms, st);
+  NsBatch* wide[kNsShapes];
+  int count = 0;
+  for (int i = 0; i < n; ++i) {
+    if (narrow_fits(shapes[i].rows, shapes[i].cols, coef, steps)) {
+      if (int rc = narrow_run(shapes[i], coef, steps, &shapes[i].out, sms, st)) return rc;
+    } else {
+      wide[count++] = &shapes[i];
+    }
+  }
+  if (count == 0) return HA_OK;
+  if (count == 1 && (wide[0]->n < 3 || wide[0]->n * wide[0]->plane_x * 6 <= kCacheBytes)) return run<OneShape>(wide, 1, coef, steps, sms, st);
+  return run<ManyShapes>(wide, count, coef, steps, sms, st);
 }
 
 }  // namespace ha

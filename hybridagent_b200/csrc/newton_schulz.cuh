@@ -26,7 +26,9 @@ struct NsBatch {
   __half* square[3];             // m x m: Gram matrices and factors
   uint32_t* counter;             // one for each matrix, zero before the run
   uint32_t* error;               // set to 1 if a wait ran out
+  int out;                       // after a run: the high plane that holds the result
 };
+constexpr int kNsShapes = 6;     // of one run
 
 // The largest |a t + b t^3 + c t^5| and |a + b t^2 + c t^4| of a step for 0 <= t <= s: how far it can
 // carry singular values up to s, and what it multiplies X by.
@@ -46,8 +48,12 @@ int ns_map(CUtensorMap* map, const __half* plane, const NsBatch& b, int box_cols
 bool narrow_fits(int64_t rows, int64_t cols, const float* coef, int steps);
 int narrow_run(const NsBatch& b, const float* coef, int steps, int* out, int sms, cudaStream_t st);
 
-// Runs `steps` Newton-Schulz steps on hi[0] (+ lo); returns in *out the index of the hi plane that
-// holds the result.
-int ns_run(const NsBatch& b, const float* coef, int steps, int* out, cudaStream_t st);
+// Stages that a shape takes at most; a run's shapes take kNsStages together.
+int ns_stages(int steps);
+constexpr int kNsStages = 128;
+
+// Runs `steps` Newton-Schulz steps on hi[0] (+ lo) of up to kNsShapes shapes, whose counters lie one after
+// another in their order.
+int ns_run(NsBatch* shapes, int n, const float* coef, int steps, cudaStream_t st);
 
 }  // namespace ha

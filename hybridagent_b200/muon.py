@@ -122,8 +122,8 @@ class ZeroOneMuon(ZeroOneAdamW):
     take Muon's and all others AdamW's.  Embeddings and output heads are usually given
     ``"use_muon": False``.  ``betas`` and ``eps`` belong to the AdamW tensors, ``weight_decay`` to both.
     ``exp_avg`` holds a Muon tensor's momentum; it has no ``exp_avg_sq``.  Workspace for the products, of
-    HYBRIDAGENT_B200_MUON_BYTES (default 2 GiB, at least the largest owned matrix's need and no more than
-    the largest group of equal shapes needs), is held for the optimizer's life."""
+    HYBRIDAGENT_B200_MUON_BYTES (default 4 GiB, at least the largest owned matrix's need and no more than
+    all of them need), is held for the optimizer's life."""
 
     state_format = "hybridagent_b200.zero1_muon/1"
     _updates = ("AdamW", "Muon")
@@ -144,12 +144,14 @@ class ZeroOneMuon(ZeroOneAdamW):
                          weight_decay=weight_decay, comm_timeout_s=comm_timeout_s, land_grads=land_grads)
         muon = [c for c in self._classes if c.muon and c.owned]
         with torch.cuda.device(self.device):
-            size = 0
+            size, budget = 0, _budget("HYBRIDAGENT_B200_MUON_BYTES", 4 << 30)
             for c in muon:
-                c.shapes = self._shape_groups(c)
-                for rows, cols, entries in c.shapes:
-                    one, need = _workspace_bytes(1, rows, cols), _workspace_bytes(len(entries), rows, cols)
-                    size = max(size, min(need, max(one, _budget("HYBRIDAGENT_B200_MUON_BYTES", 2 << 30))))
+                shapes = [tuple(self.params[i].shape) for i in c.owned]
+                # equal shapes follow one another: they run together
+                c.order = np.asarray(sorted(range(len(shapes)), key=lambda k: shapes[k]), dtype=np.int64)
+                c.shapes = np.ascontiguousarray([shapes[k] for k in c.order], dtype=np.int64)
+                need = sum(_workspace_bytes(1, *s) for s in shapes)
+                size = max(size, min(need, max(budget, *(_workspace_bytes(1, *s) for s in set(shapes)), 0)))
                 c.neg_lr = np.asarray([-(self.lrs[i] * self._factor(*self.params[i].shape)) for i in c.owned],
                                       dtype=np.float32)
             self._muon_ws = torch.empty(size, dtype=torch.uint8, device=self.device) if size else None
@@ -173,13 +175,6 @@ class ZeroOneMuon(ZeroOneAdamW):
             return math.sqrt(max(1.0, rows / cols))
         return 1.0
 
-    def _shape_groups(self, c) -> list[tuple[int, int, np.ndarray]]:
-        """(rows, cols, table entries) of the owned matrices of equal shape, which run together."""
-        groups: dict[tuple[int, int], list[int]] = {}
-        for k, i in enumerate(c.owned):
-            groups.setdefault(tuple(self.params[i].shape), []).append(k)
-        return [(rows, cols, np.asarray(entries, dtype=np.int64)) for (rows, cols), entries in groups.items()]
-
     def _check_muon_status(self, wait: bool = False) -> None:
         """Raises if an earlier step's products gave up waiting (its matrices were then not updated)."""
         if self._muon_event is not None and (wait or self._muon_event.query()):
@@ -191,20 +186,18 @@ class ZeroOneMuon(ZeroOneAdamW):
                                    "that step were not updated")
 
     def _update_muon(self, c, sc: _lib.AdamwScalars, changed_only: bool, p2p: bool) -> None:
-        """The Muon update of class c's owned matrices that have a gradient, shape by shape."""
+        """The Muon update of class c's owned matrices that have a gradient."""
         self._check_muon_status()
         ms = _lib.MuonScalars(np.float32(self.momentum), np.float32(1.0 - self.momentum), int(self.nesterov),
                               sc.use_decay, sc.clip, sc.clip_mult)
-        for rows, cols, entries in c.shapes:
-            table = np.ascontiguousarray(c.table.np[entries])
-            count = int(np.count_nonzero(table["grad"]))
-            if not count:
-                continue
-            _lib.call("ha_muon_step", _lib.np_ptr(table), len(table), rows, cols, c.code, ctypes.byref(ms),
-                      ctypes.byref(self._ns), int(changed_only), ctypes.byref(c.peers) if p2p else None,
-                      c.changed_dev.data_ptr() if changed_only else None, self._muon_status.data_ptr(),
-                      self._muon_ws.data_ptr(), self._muon_ws.numel(), self._stream())
-            self.launches += 3 * (1 + self._ns.steps)  # at least: more where the workspace or a slice splits them
+        table = np.ascontiguousarray(c.table.np[c.order])
+        _lib.call("ha_muon_step", _lib.np_ptr(table), _lib.np_ptr(c.shapes), len(table), c.code, ctypes.byref(ms),
+                  ctypes.byref(self._ns), int(changed_only), ctypes.byref(c.peers) if p2p else None,
+                  c.changed_dev.data_ptr() if changed_only else None, self._muon_status.data_ptr(),
+                  self._muon_ws.data_ptr(), self._muon_ws.numel(), self._stream())
+        # momentum, load and weights of each shape, and one run of the products: more where the workspace or a
+        # launch's parameters split them
+        self.launches += 3 * len({tuple(s) for s in c.shapes.tolist()}) + 1
         self._muon_status_host.copy_(self._muon_status, non_blocking=True)
         self._muon_event = torch.cuda.Event()
         self._muon_event.record()

@@ -271,8 +271,9 @@ typedef struct ha_muon_scalars {
   float clip_mult;
 } ha_muon_scalars;
 
-/* Workspace bytes with which `batch` matrices of rows x cols (at most 32768 of them) pass at once.  The calls
- * below take any size from that of one matrix up and pass through it several times if they must. */
+/* Workspace bytes with which `batch` matrices of rows x cols (at most 4096 of them) pass at once.  The calls
+ * below take any size from that of one matrix up (of their largest shape) and pass through it several times
+ * if they must. */
 int ha_orthogonalize_workspace(int64_t batch, int64_t rows, int64_t cols, size_t* out);
 
 /* Orthogonalises `batch` contiguous row-major matrices of rows x cols: singular values towards 1, singular
@@ -282,15 +283,16 @@ int ha_orthogonalize_workspace(int64_t batch, int64_t rows, int64_t cols, size_t
 int ha_orthogonalize(const void* src, int src_dtype, void* dst, int64_t batch, int64_t rows, int64_t cols,
                      const ha_ns_params* ns, void* workspace, size_t workspace_bytes, void* stream);
 
-/* One Muon step of `n` matrices of rows x cols (a HOST table, read before the call returns; entries
- * with grad == 0 are skipped):
+/* One Muon step of `n` matrices (a HOST table, read before the call returns; entries with grad == 0 are
+ * skipped); entry i has h_shapes[2i] rows and h_shapes[2i + 1] columns, and entries of equal shape that follow one
+ * another run together:
  *     M <- mu M + (1 - mu) g;  U = direction;  O = Newton-Schulz(U);  W <- W decay + neg_lr O
  * with M = exp_avg, W = master, and the copy of W in grad_dtype at `param` (16-bit types; for HA_F32
  * the master is the parameter).  exp_avg_sq, rc1 and rc2 are not read; neg_lr includes any factor for
  * the shape.  changed_only: 16-bit copies are stored by changed sectors, under ha_adamw_step_delta's
  * conditions; peers (may be NULL) and d_changed_groups as there.  Should a wait inside the products
  * run out, the weights stay as they are and *d_status (device, may be NULL) becomes 1. */
-int ha_muon_step(const ha_tensor* h_tensors, int64_t n, int64_t rows, int64_t cols, int grad_dtype,
+int ha_muon_step(const ha_tensor* h_tensors, const int64_t* h_shapes, int64_t n, int grad_dtype,
                  const ha_muon_scalars* sc, const ha_ns_params* ns, int changed_only, const ha_peers* peers,
                  unsigned long long* d_changed_groups, uint32_t* d_status, void* workspace, size_t workspace_bytes,
                  void* stream);

@@ -458,7 +458,8 @@ def test_muon_step_writes_the_peers_copies(code, changed_only):
     ws = torch.empty(muon._workspace_bytes(n, rows, cols), dtype=torch.uint8, device="cuda")
     count = torch.zeros(1, dtype=torch.int64, device="cuda")
     status = torch.zeros(1, dtype=torch.int32, device="cuda")
-    _lib.call("ha_muon_step", _lib.np_ptr(tab), n, rows, cols, code, ctypes.byref(sc), ctypes.byref(ns), changed_only,
+    shapes = np.asarray([[rows, cols]] * n, dtype=np.int64)
+    _lib.call("ha_muon_step", _lib.np_ptr(tab), _lib.np_ptr(shapes), n, code, ctypes.byref(sc), ctypes.byref(ns), changed_only,
               ctypes.byref(peers), count.data_ptr(), status.data_ptr(), ws.data_ptr(), ws.numel(),
               torch.cuda.current_stream().cuda_stream)
     torch.cuda.synchronize()

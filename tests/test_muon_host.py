@@ -25,7 +25,7 @@ def test_workspace_grows_with_the_batch_and_holds_the_planes():
         assert _bytes(0, rows, cols) == one < two < many
         assert many < 41 * one
         assert one > 3 * 2 * rows * cols  # at least the high planes before and after a step, and the low plane
-        assert _bytes(10**9, rows, cols) == _bytes(32768, rows, cols)  # the most that pass at once
+        assert _bytes(10**9, rows, cols) == _bytes(4096, rows, cols)  # the most that pass at once
     for bad in ((0, 5), (5, 0), (-1, 4), (1 << 25, 4), (1 << 24, 1 << 20)):
         with pytest.raises(_lib.HAError, match="matrices of"):
             _bytes(1, *bad)
@@ -77,8 +77,10 @@ def test_orthogonalize_accepts_usual_coefficients_and_nothing_to_do():
 def test_muon_step_refuses():
     sc = _lib.MuonScalars(0.95, 0.05, 1, 0, 0, 1.0)
 
-    def call(tab, n=None, rows=64, cols=96, code=_lib.HA_BF16, scalars=sc, peers=None, ws=WS):
-        _lib.call("ha_muon_step", None if tab is None else _lib.np_ptr(tab), len(tab) if n is None else n, rows, cols, code,
+    def call(tab, n=None, rows=64, cols=96, code=_lib.HA_BF16, scalars=sc, peers=None, ws=WS, no_shapes=False):
+        shapes = np.asarray([[rows, cols]] * 1, dtype=np.int64)
+        _lib.call("ha_muon_step", None if tab is None else _lib.np_ptr(tab), None if no_shapes else _lib.np_ptr(shapes),
+                  len(tab) if n is None else n, code,
                   None if scalars is None else ctypes.byref(scalars), ctypes.byref(_ns()), 0,
                   None if peers is None else ctypes.byref(peers), None, None, ws, _bytes(1, 64, 96), None)
 
@@ -96,6 +98,8 @@ def test_muon_step_refuses():
         call(entry(), scalars=None)
     with pytest.raises(_lib.HAError, match="NULL table"):
         call(None, n=1)
+    with pytest.raises(_lib.HAError, match="NULL table"):
+        call(entry(), no_shapes=True)
     with pytest.raises(_lib.HAError, match="matrices of"):
         call(entry(), rows=0)
     for kw in (dict(numel=64 * 95), dict(master=0), dict(exp_avg=0), dict(param=0)):
