@@ -311,7 +311,10 @@ __global__ void __launch_bounds__(kThreads)
   static_assert(!(DELTA && DT == HA_F32), "fp32 parameters are their own masters: always written");
   __shared__ uint32_t stored_in_cta;
   if (*error != 0) {  // a wait of the products ran out: the weights stay as they are
-    if (threadIdx.x == 0 && status != nullptr) atomicExch(status, 1u);
+    if (threadIdx.x == 0 && status != nullptr) {
+      *static_cast<volatile uint32_t*>(status) = 1u;
+      __threadfence_system();
+    }
     return;
   }
   const ha_tensor& t = s.t[blockIdx.y];
@@ -329,10 +332,18 @@ __global__ void __launch_bounds__(kThreads)
     if (use_decay) w = __fmul_rn(w, decay);
     return __fmaf_rn(lr, o, w);
   };
+  // Row and column of an element, 32-bit from the chunk's first one on (a chunk has 2^14 elements).
+  const int64_t row0 = begin / sh.cols;
+  const uint32_t col0 = uint32_t(begin - row0 * sh.cols), cols = uint32_t(sh.cols);
+  auto place = [&](int64_t k, uint32_t& c) {
+    const uint32_t at = col0 + uint32_t(k - begin), r = at / cols;
+    c = at - r * cols;
+    return x + (row0 + r) * sh.ld + c;
+  };
   auto one = [&](int64_t k) {
-    const int64_t r = k / sh.cols, c = k - r * sh.cols;
+    uint32_t c;
     const float before = master[k];
-    const float a = update(before, __half2float(x[r * sh.ld + c]));
+    const float a = update(before, __half2float(*place(k, c)));
     master[k] = a;
     if constexpr (DT != HA_F32) {
       const uint16_t w = Elem<DT>::narrow(a);
@@ -355,9 +366,10 @@ __global__ void __launch_bounds__(kThreads)
         e[u] = base + 4 * (int64_t(threadIdx.x) + int64_t(u) * kThreads);
         if (e[u] + 4 <= end) {
           ms[u] = load4_f32(master, e[u]);
-          int64_t r = e[u] / sh.cols, c = e[u] - r * sh.cols;
+          uint32_t c;
+          const __half* o_at = place(e[u], c);
           if (vec_x) {
-            const uint2 w = *reinterpret_cast<const uint2*>(x + r * sh.ld + c);
+            const uint2 w = *reinterpret_cast<const uint2*>(o_at);
             const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&w.x));
             const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&w.y));
             o[u] = make_float4(a.x, a.y, b.x, b.y);
@@ -365,8 +377,8 @@ __global__ void __launch_bounds__(kThreads)
             float v[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              v[i] = __half2float(x[r * sh.ld + c]);
-              if (++c == sh.cols) c = 0, ++r;
+              v[i] = __half2float(*o_at++);
+              if (++c == cols) c = 0, o_at += sh.ld - sh.cols;
             }
             o[u] = make_float4(v[0], v[1], v[2], v[3]);
           }

@@ -155,9 +155,8 @@ class ZeroOneMuon(ZeroOneAdamW):
                 c.neg_lr = np.asarray([-(self.lrs[i] * self._factor(*self.params[i].shape)) for i in c.owned],
                                       dtype=np.float32)
             self._muon_ws = torch.empty(size, dtype=torch.uint8, device=self.device) if size else None
-            self._muon_status = torch.zeros(1, dtype=torch.int32, device=self.device)
-            self._muon_status_host = torch.zeros(1, dtype=torch.int32, pin_memory=True)
-            self._muon_event: torch.cuda.Event | None = None
+            # set by a step whose products gave up; pinned host memory, which the GPU writes itself
+            self._muon_status = torch.zeros(1, dtype=torch.int32, pin_memory=True)
             torch.cuda.current_stream().synchronize()
 
     def _takes_muon(self, parameter: torch.Tensor, group: dict) -> bool:
@@ -175,19 +174,11 @@ class ZeroOneMuon(ZeroOneAdamW):
             return math.sqrt(max(1.0, rows / cols))
         return 1.0
 
-    def _check_muon_status(self, wait: bool = False) -> None:
-        """Raises if an earlier step's products gave up waiting (its matrices were then not updated)."""
-        if self._muon_event is not None and (wait or self._muon_event.query()):
-            if wait:
-                self._muon_event.synchronize()
-            self._muon_event = None
-            if int(self._muon_status_host[0]) != 0:
-                raise RuntimeError("Muon step: a wait inside the Newton-Schulz products ran out; the matrices of "
-                                   "that step were not updated")
-
     def _update_muon(self, c, sc: _lib.AdamwScalars, changed_only: bool, p2p: bool) -> None:
         """The Muon update of class c's owned matrices that have a gradient."""
-        self._check_muon_status()
+        if int(self._muon_status[0]) != 0:
+            raise RuntimeError("Muon step: a wait inside the Newton-Schulz products ran out; the matrices of that "
+                               "step were not updated")
         ms = _lib.MuonScalars(np.float32(self.momentum), np.float32(1.0 - self.momentum), int(self.nesterov),
                               sc.use_decay, sc.clip, sc.clip_mult)
         table = np.ascontiguousarray(c.table.np[c.order])
@@ -198,9 +189,6 @@ class ZeroOneMuon(ZeroOneAdamW):
         # momentum, load and weights of each shape, and one run of the products: more where the workspace or a
         # launch's parameters split them
         self.launches += 3 * len({tuple(s) for s in c.shapes.tolist()}) + 1
-        self._muon_status_host.copy_(self._muon_status, non_blocking=True)
-        self._muon_event = torch.cuda.Event()
-        self._muon_event.record()
 
     def state_summary(self) -> str:
         n = sum(len(c.layout.indices) for c in self._classes if c.muon)

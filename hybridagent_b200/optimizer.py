@@ -591,11 +591,7 @@ class ZeroOneAdamW:
     def _param_versions(self) -> np.ndarray:
         """(address, torch version) of every parameter: a re-bound or in-place-modified
         parameter shows up as a change."""
-        out = np.zeros((len(self.params), 2), dtype=np.int64)
-        for i, p in enumerate(self.params):
-            out[i, 0] = p.data_ptr()
-            out[i, 1] = p._version
-        return out
+        return np.array([(p.data_ptr(), p._version) for p in self.params], dtype=np.int64)
 
     def _master_versions(self) -> list[int]:
         """Torch version of each class's packed master buffer (the masters are views of it, so
@@ -1131,8 +1127,10 @@ class ZeroOneAdamW:
                 partial = self._read_local(self._lland_out[:n_slots], self._lland_out_host[:n_slots])
                 self.land_norm_steps += 1
             else:
+                if self.world == 1:  # the next update's tables serve the sums too: one upload
+                    self._stage_step()
                 # (the contiguous copies of strided gradients must outlive the launches)
-                keep = None if reuse else self._launch_sumsq()  # noqa: F841
+                keep = None if reuse else self._launch_sumsq(upload=self.world > 1)  # noqa: F841
                 if self.world > 1 and reuse:  # the exchange's square sums, one per class and round
                     self._comm.all_reduce_sum(self._norm_rounds, HA_F64)
                     self._stage_step()
@@ -1144,21 +1142,23 @@ class ZeroOneAdamW:
                     partial = self._comm.read(self._norm_buf, self._norm_host,
                                               "all-reduce(sum) of the norm").tolist()
                 else:
-                    partial = self._read_local(self._norm_buf, self._norm_host)
+                    partial = self._read_local(self._norm_buf, self._norm_host, stage=False)
         total = np.float32(sum(partial))  # the reference's total is an fp32 tensor
         norm = float(np.sqrt(total))      # float(total.sqrt()), optimizer.py:154
         if max_norm > 0 and norm > max_norm:
             self._pending_clip = float(max_norm) / (norm + 1e-6)  # optimizer.py:156
         return norm
 
-    def _launch_sumsq(self) -> list:
-        """One ``ha_grad_sumsq`` per dtype class over its owned gradients into ``_norm_buf``;
-        returns the gradient lists, whose contiguous copies must outlive the launches."""
+    def _launch_sumsq(self, upload: bool) -> list:
+        """One ``ha_grad_sumsq`` per dtype class over its owned gradients into ``_norm_buf``, with
+        the tables uploaded first unless they hold these gradients already; returns the
+        gradient lists, whose contiguous copies must outlive the launches."""
         keep = []
         for k, c in enumerate(self._classes):
             grads, ptrs = self._cached_grads(k, c)
             keep.append(grads)
-            self._upload_table(c, ptrs, advance=False)
+            if upload:
+                self._upload_table(c, ptrs, advance=False)
         self._phase("sumsq", True)
         for k, c in enumerate(self._classes):
             chunks, n = c.sumsq_chunks
@@ -1168,13 +1168,14 @@ class ZeroOneAdamW:
         self._phase("sumsq", False)
         return keep
 
-    def _read_local(self, dev: torch.Tensor, host: torch.Tensor) -> list:
+    def _read_local(self, dev: torch.Tensor, host: torch.Tensor, stage: bool = True) -> list:
         """World size 1: copies the fp64 sums to pinned host memory, stages the next step's
-        tables while the copy is in flight, and returns the sums."""
+        tables while the copy is in flight (if they are not yet), and returns the sums."""
         host.copy_(dev, non_blocking=True)
         ev = torch.cuda.Event()
         ev.record()
-        self._stage_step()
+        if stage:
+            self._stage_step()
         ev.synchronize()
         return host.tolist()
 
@@ -1255,7 +1256,7 @@ class ZeroOneAdamW:
             self._phase("adamw", True)
             ce_gather = p2p and self.gather_mode == "ce"
             main = torch.cuda.current_stream()
-            for c, sc in launches:
+            for c, sc in sorted(launches, key=lambda item: not item[0].muon):  # the longest work first
                 chunks, n = c.adamw_chunks
                 if c.changed_event is not None and c.changed_event.query():  # the last count has landed
                     c.last_changed = int(c.changed_host[0])
