@@ -251,10 +251,10 @@ __global__ void __launch_bounds__(kThreads) load_kernel(const __grid_constant__ 
   }
 }
 
-// The orthogonalised matrices as bf16 (NaN if a wait of the products ran out), eight elements of the
-// packed result per thread, so that odd row lengths cost unaligned loads but no narrow stores.
+// The orthogonalised matrices as bf16 (`rounded`: which they are; NaN if a wait of the products ran out), eight
+// elements of the packed result per thread, so that odd row lengths cost unaligned loads but no narrow stores.
 __global__ void __launch_bounds__(kThreads)
-    store_kernel(const __half* x, Shape sh, int64_t total, uint16_t* out, const uint32_t* error) {
+    store_kernel(const __half* x, Shape sh, bool rounded, int64_t total, uint16_t* out, const uint32_t* error) {
   const bool bad = *error != 0;
   const int64_t numel = sh.rows * sh.cols;
   const bool vec = (sh.cols & 7) == 0;
@@ -288,8 +288,9 @@ __global__ void __launch_bounds__(kThreads)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&b[i]));
-      b[i] = bad ? 0x7fff7fffu
-                 : uint32_t(Elem<HA_BF16>::narrow(f.x * (1.0f / kScaleX))) |
+      b[i] = bad       ? 0x7fff7fffu
+             : rounded ? b[i]
+                       : uint32_t(Elem<HA_BF16>::narrow(f.x * (1.0f / kScaleX))) |
                        (uint32_t(Elem<HA_BF16>::narrow(f.y * (1.0f / kScaleX))) << 16);
     }
     if (e + 8 <= total && (reinterpret_cast<uintptr_t>(out) & 15) == 0) {
@@ -521,7 +522,7 @@ struct Pass {
   int run(const ha_ns_params& ns, cudaStream_t st) {
     for (int i = 0; i < groups; ++i) batches[i] = group[i].b;
     const int rc = ns_run(batches, groups, ns.coef, ns.steps, st);
-    for (int i = 0; i < groups; ++i) group[i].b.out = batches[i].out;
+    for (int i = 0; i < groups; ++i) group[i].b.out = batches[i].out, group[i].b.rounded = batches[i].rounded;
     return rc;
   }
 };
@@ -553,11 +554,16 @@ int orthogonalize(const void* src, void* dst, int64_t batch, int64_t rows, int64
       load_kernel<<<dim3(load_grid(g.b), m), kThreads, 0, st>>>(PlainSource<DT>{x + k * numel, numel}, sh, g.n_partials,
                                                                part, ns.eps, int(k), g.b.hi[0], g.b.lo, g.b.counter);
     }
+    // rows of 16-byte pieces: the last product stores the result itself
+    uint16_t* out = static_cast<uint16_t*>(dst) + i * numel;
+    g.b.bf16 = true;
+    if ((cols & 7) == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0) g.b.dst = out;
     int rc = check_launch("ha_orthogonalize (load)");
     if (rc == HA_OK) rc = pass.run(ns, st);
     if (rc != HA_OK) return rc;
+    if (g.b.out < 0) continue;
     store_kernel<<<dim3(unsigned((n * numel + kLoadChunk - 1) / kLoadChunk)), kThreads, 0, st>>>(
-        g.b.hi[g.b.out], sh, n * numel, static_cast<uint16_t*>(dst) + i * numel, g.b.error);
+        g.b.hi[g.b.out], sh, g.b.rounded, n * numel, out, g.b.error);
     rc = check_launch("ha_orthogonalize (store)");
     if (rc != HA_OK) return rc;
   }

@@ -26,9 +26,7 @@
 // of jobs (a stage, that is one product, of some matrices of one shape), whose tiles the CTAs take in turn; a tile
 // waits until all tiles of the previous stage of its matrix are stored (a counter per matrix in global memory), so
 // matrices need not wait for one another and a job's last tiles run beside the next one's first.  Jobs of several
-// shapes alternate, so that one shape's tiles fill the time in which another's results travel; of a batch that
-// does not fit L2, X is multiplied a few matrices at a time, each followed soon by its Gram matrix, which then finds
-// X in L2 and gives the tensor cores work while the next X streams through.  A job waits only for jobs before it
+// shapes alternate, so that one shape's tiles fill the time in which another's results travel.  A job waits only for jobs before it
 // in the list, and the launch is cooperative: all CTAs are resident, so the waits end.
 //
 // In a CTA, warp 0 feeds a ring of 128-byte-swizzled operand tiles by TMA, one thread of warp 1 issues the
@@ -55,7 +53,6 @@ constexpr int kBM = 128;           // rows of a CTA's part of a tile: the TMEM l
 constexpr int kBK = 64;            // K elements of a ring slot: one 128-byte swizzle row
 constexpr int kGemmThreads = 416;  // operands, MMA, addends, stores; eight epilogue warps; stores
 constexpr int kPreciseSteps = 3;
-constexpr int64_t kCacheBytes = 64 << 20;  // planes that stay in L2 (126 MB) beside the rest of a stage
 constexpr int kHalf = kBM * kBK * 2;  // bytes of one operand's part of a slot
 constexpr int kSlot = 2 * kHalf;
 constexpr int kSlots = 5;
@@ -69,7 +66,8 @@ constexpr int kGemmSmem = kSlots * kSlot + kBlocks * 2 * kBlock + 1024;  // + al
 //   kPoly       the same after adding add * addend and `diag` on the diagonal
 //   kPrecise    added to add * low, stored as high and low plane
 //   kPlain      stored
-enum Epilogue { kSymmetric, kPoly, kPrecise, kPlain };
+//   kFinal      stored as bf16
+enum Epilogue { kSymmetric, kPoly, kPrecise, kPlain, kFinal };
 
 // Tensor maps of a run: per buffer, the boxes it is read and written in.
 enum Map {
@@ -80,7 +78,8 @@ enum Map {
   kMapSq = 7,       // + 0 .. 2: square matrices, operand tiles
   kMapSqOut = 10,   // + 0 .. 2: epilogue blocks
   kMapSqMirror = 13,  // + 0 .. 2: mirrored blocks, 32 x 128
-  kMaps = 16
+  kMapDst = 16,       // the caller's matrices, epilogue blocks
+  kMaps = 17
 };
 
 struct Stage {
@@ -106,9 +105,11 @@ struct RunArgsOf {
   int jobs;
   uint32_t* counter;  // one for each matrix
   uint32_t* error;
+  uint16_t* dst;      // the caller's matrices, if a stage writes them
+  int64_t dst_elems;
 };
 constexpr int kMaxStages = 3 * HA_NS_MAX_STEPS + 2;  // of one shape
-constexpr int kManyShapes = kNsShapes, kManyStages = kNsStages, kManyJobs = 1024;
+constexpr int kManyShapes = kNsShapes, kManyStages = kNsStages, kManyJobs = kNsStages;
 using OneShape = RunArgsOf<1, kMaxStages, kMaxStages>;
 using ManyShapes = RunArgsOf<kManyShapes, kManyStages, kManyJobs>;
 static_assert(sizeof(ManyShapes) <= 32000, "kernel parameters");
@@ -228,7 +229,12 @@ __device__ __forceinline__ bool epilogue(const Stage& g, const Job& job, Warp& w
           if (col + 2 * j == row) x += diag;
           if (col + 2 * j + 1 == row) y += diag;
         }
-        out[j] = pack_half2(x, y);
+        if (EPI == kFinal) {
+          const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+          out[j] = *reinterpret_cast<const uint32_t*>(&h);
+        } else {
+          out[j] = pack_half2(x, y);
+        }
         if (EPI == kPrecise) {
           const float2 a = unpack_half2(out[j]);
           low[j] = pack_half2((x - a.x) * kScaleLo, (y - a.y) * kScaleLo);
@@ -505,7 +511,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1) newton_schulz_kernel(const __
         case kSymmetric: ok = epilogue<CG, kSymmetric>(g, job, w, sh); break;
         case kPoly: ok = epilogue<CG, kPoly>(g, job, w, sh); break;
         case kPrecise: ok = epilogue<CG, kPrecise>(g, job, w, sh); break;
-        default: ok = epilogue<CG, kPlain>(g, job, w, sh); break;
+        case kPlain: ok = epilogue<CG, kPlain>(g, job, w, sh); break;
+        default: ok = epilogue<CG, kFinal>(g, job, w, sh); break;
       }
       w.walk.pass(job.count * g.per_matrix);
     }
@@ -516,6 +523,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1) newton_schulz_kernel(const __
     const uint64_t t0 = global_ns();
     while (global_ns() - t0 < 2000000) {
     }
+    if (p.dst != nullptr)
+      for (int64_t e = threadIdx.x; e < p.dst_elems; e += kGemmThreads) p.dst[e] = 0x7fff;
     __syncthreads();
   }
   tc_fence_before();
@@ -603,6 +612,8 @@ int make_maps(const NsBatch& b, CUtensorMap* maps) {
     operand(kMapXmn + i, x, 64);
     block(kMapXout + i, x);
   }
+  if (b.dst != nullptr)
+    block(kMapDst, Operand{reinterpret_cast<const __half*>(b.dst), b.rows, b.cols, b.cols, b.rows * b.cols});
   block(kMapLow, Operand{b.lo, b.rows, b.cols, b.ld_x, b.plane_x});
   for (int i = 0; i < 3; ++i) {
     const Operand q{b.square[i], b.m, b.m, b.ld_g, b.plane_g};
@@ -675,7 +686,17 @@ int make_stages(NsBatch* shape, const float* coef, int steps, int map0, int coun
     s += pair ? 2 : 1;
     g->keep_low = s < kPreciseSteps && s < steps;  // the next step reads it
   }
+  Stage& last = stages[count - 1];
   shape->out = cur;
+  shape->rounded = b.bf16 && last.epilogue == kPlain;
+  if (shape->rounded) {
+    last.epilogue = kFinal;
+    last.scale /= kScaleX;
+    if (b.dst != nullptr) {
+      last.map_out = uint8_t(map0 + kMapDst);
+      shape->out = -1;
+    }
+  }
   return count;
 }
 
@@ -706,33 +727,14 @@ struct Placed {
   Job job;
   double at;
 };
-int place(const Stage* stages, int first_stage, int count, const NsBatch& b, int workers, Placed* out, int room) {
+int place(const Stage* stages, int first_stage, int count, const NsBatch& b, Placed* out) {
   int n = 0;
   double total = 0.0, done = 0.0;
   auto cost = [&](int s) { return double(stages[s].per_matrix) * ((stages[s].K + kBK - 1) / kBK); };
-  for (int s = 0; s < count; ++s) total += cost(s) * double(b.n);
-  auto put = [&](int s, int64_t first, int64_t matrices) {
-    out[n++] = Placed{Job{uint16_t(first_stage + s), uint16_t(first), uint16_t(matrices), 0}, done / total};
-    done += cost(s) * double(matrices);
-  };
+  for (int s = 0; s < count; ++s) total += cost(s);
   for (int s = 0; s < count; ++s) {
-    // a product with X and the Gram matrix of its result, a few matrices at a time if the planes exceed L2
-    const bool x = stages[s].epilogue >= kPrecise;
-    int64_t chunk = b.n;
-    if (x && s + 1 < count && b.n * b.plane_x * 6 > kCacheBytes) {
-      chunk = (2 * workers + stages[s].per_matrix - 1) / stages[s].per_matrix;
-      if (chunk * 64 < b.n) chunk = (b.n + 63) / 64;
-    }
-    const int64_t chunks = (b.n + chunk - 1) / chunk;
-    if (chunks < 3 || n + 2 * chunks + (count - s) > room) {
-      put(s, 0, b.n);
-      continue;
-    }
-    for (int64_t c = 0; c <= chunks; ++c) {  // the Gram matrices one chunk behind
-      if (c < chunks) put(s, c * chunk, c * chunk + chunk < b.n ? chunk : b.n - c * chunk);
-      if (c > 0) put(s + 1, (c - 1) * chunk, c < chunks ? chunk : b.n - (c - 1) * chunk);
-    }
-    ++s;
+    out[n++] = Placed{Job{uint16_t(first_stage + s), 0, uint16_t(b.n), 0}, done / total};
+    done += cost(s);
   }
   return n;
 }
@@ -793,13 +795,14 @@ int run(NsBatch** shapes, int n, const float* coef, int steps, int sms, cudaStre
   if (cg == 2) cost(2);
   int jobs = 0;
   for (int i = 0; i < n; ++i)
-    jobs += place(p.stage + first[i], first[i], first[i + 1] - first[i], *shapes[i], sms / cg, list + jobs,
-                  (kRoom - jobs) / (n - i));
+    jobs += place(p.stage + first[i], first[i], first[i + 1] - first[i], *shapes[i], list + jobs);
   std::stable_sort(list, list + jobs, [](const Placed& a, const Placed& b) { return a.at < b.at; });
   for (int q = 0; q < jobs; ++q) p.job[q] = list[q].job;
   p.jobs = jobs;
   p.counter = shapes[0]->counter;
   p.error = shapes[0]->error;
+  p.dst = n == 1 && shapes[0]->out < 0 ? shapes[0]->dst : nullptr;
+  p.dst_elems = shapes[0]->n * shapes[0]->rows * shapes[0]->cols;
   return cg == 1 ? launch<1>(p, sms, st) : launch<2>(p, sms, st);
 }
 
@@ -866,13 +869,13 @@ int ns_run(NsBatch* shapes, int n, const float* coef, int steps, cudaStream_t st
   int count = 0;
   for (int i = 0; i < n; ++i) {
     if (narrow_fits(shapes[i].rows, shapes[i].cols, coef, steps)) {
-      if (int rc = narrow_run(shapes[i], coef, steps, &shapes[i].out, sms, st)) return rc;
+      if (int rc = narrow_run(&shapes[i], coef, steps, sms, st)) return rc;
     } else {
       wide[count++] = &shapes[i];
     }
   }
   if (count == 0) return HA_OK;
-  if (count == 1 && (wide[0]->n < 3 || wide[0]->n * wide[0]->plane_x * 6 <= kCacheBytes)) return run<OneShape>(wide, 1, coef, steps, sms, st);
+  if (count == 1) return run<OneShape>(wide, 1, coef, steps, sms, st);
   return run<ManyShapes>(wide, count, coef, steps, sms, st);
 }
 

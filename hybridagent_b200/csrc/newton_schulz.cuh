@@ -26,7 +26,10 @@ struct NsBatch {
   __half* square[3];             // m x m: Gram matrices and factors
   uint32_t* counter;             // one for each matrix, zero before the run
   uint32_t* error;               // set to 1 if a wait ran out
-  int out;                       // after a run: the high plane that holds the result
+  bool bf16;                     // the result is wanted as bf16 (a run of this shape alone) ...
+  uint16_t* dst;                 // ... in packed matrices with 16-byte aligned rows, if set
+  int out;                       // after a run: the high plane that holds the result, or -1 if dst does
+  bool rounded;                  // after a run: the result is bf16 (not 2^12 times it in fp16)
 };
 constexpr int kNsShapes = 6;     // of one run
 
@@ -46,7 +49,7 @@ int ns_map(CUtensorMap* map, const __half* plane, const NsBatch& b, int box_cols
 
 // Matrices whose shorter side is at most 128, if the steps' factors fit (newton_schulz_narrow.cu).
 bool narrow_fits(int64_t rows, int64_t cols, const float* coef, int steps);
-int narrow_run(const NsBatch& b, const float* coef, int steps, int* out, int sms, cudaStream_t st);
+int narrow_run(NsBatch* shape, const float* coef, int steps, int sms, cudaStream_t st);
 
 // Stages that a shape takes at most; a run's shapes take kNsStages together.
 int ns_stages(int steps);

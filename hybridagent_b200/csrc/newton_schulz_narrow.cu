@@ -39,11 +39,14 @@ constexpr float kScaleS = 32.0f;           // planes of S: its elements reach th
 
 struct NarrowArgs {
   CUtensorMap hi[2], lo;    // blocks of 64 columns x 128 rows (m rounded up to 16 of them if wide)
+  CUtensorMap dst;          // the same of the caller's matrices, which take the result if `direct`
   int m, n;                 // shorter and longer side
-  int tall, cluster, steps;
+  int tall, cluster, steps, bf16, direct;
   uint32_t ends;            // bit s: a part ends after step s
   float coef[3 * HA_NS_MAX_STEPS];
   uint32_t* error;
+  uint16_t* out;            // the caller's matrices (`direct`)
+  int64_t out_elems;
 };
 
 struct Bars {
@@ -372,6 +375,7 @@ __global__ void __launch_bounds__(kThreadsN, 1) narrow_kernel(const __grid_const
   int stored = 0;
   const uint32_t idesc = p.tall ? f16_idesc(128, np, false, false) : f16_idesc(128, 64, false, true);
   const bool both = s1 < p.steps;  // X goes on: high and low plane
+  const bool bf16 = p.bf16 && !both, direct = p.direct && !both;
   auto issue = [&](int i) {  // by warp 0: the products of piece i
     const int slot = i % slots;
     wait_full(slot);
@@ -429,6 +433,10 @@ __global__ void __launch_bounds__(kThreadsN, 1) narrow_kernel(const __grid_const
           const float2 f = __half22float2(q);
           const __half2 r = __floats2half2_rn((x - f.x) * kScaleLo, (y - f.y) * kScaleLo);
           h[k] = *reinterpret_cast<const uint32_t*>(&q);
+          if (bf16) {
+            const __nv_bfloat162 w = __floats2bfloat162_rn(x * (1.0f / kScaleX), y * (1.0f / kScaleX));
+            h[k] = *reinterpret_cast<const uint32_t*>(&w);
+          }
           l[k] = *reinterpret_cast<const uint32_t*>(&r);
         }
         const uint32_t at = stage + plane_at(row, half * 32 + 8 * j);
@@ -442,7 +450,7 @@ __global__ void __launch_bounds__(kThreadsN, 1) narrow_kernel(const __grid_const
       if (warp == 0 && elect_one()) {
         tc_fence_after();
         const int at = (piece0 + i) * span, x = p.tall ? 64 * blk : at, y = p.tall ? at : 0;
-        tma_store_3d(&p.hi[plane ^ 1], stage, x, y, z);
+        tma_store_3d(direct ? &p.dst : &p.hi[plane ^ 1], stage, x, y, z);
         if (both) tma_store_3d(&p.lo, stage + kHalfPlane, x, y, z);
         tma_store_commit();
       }
@@ -459,6 +467,8 @@ __global__ void __launch_bounds__(kThreadsN, 1) narrow_kernel(const __grid_const
     const uint64_t t0 = global_ns();
     while (global_ns() - t0 < 2000000) {
     }
+    if (p.direct)
+      for (int64_t e = threadIdx.x; e < p.out_elems; e += kThreadsN) p.out[e] = 0x7fff;
   }
   tc_fence_before();
   __syncthreads();
@@ -497,15 +507,26 @@ bool narrow_fits(int64_t rows, int64_t cols, const float* coef, int steps) {
   return (rows < cols ? rows : cols) <= 128 && cut_parts(coef, steps, &ends, &parts);
 }
 
-int narrow_run(const NsBatch& b, const float* coef, int steps, int* out, int sms, cudaStream_t st) {
+int narrow_run(NsBatch* shape, const float* coef, int steps, int sms, cudaStream_t st) {
+  const NsBatch& b = *shape;
   NarrowArgs p{};
   const int box = b.rows > b.cols ? 128 : (int(b.m) + 15) & ~15;
   int rc = ns_map(&p.hi[0], b.hi[0], b, 64, box), parts = 0;
   if (rc == HA_OK) rc = ns_map(&p.hi[1], b.hi[1], b, 64, box);
   if (rc == HA_OK) rc = ns_map(&p.lo, b.lo, b, 64, box);
+  p.bf16 = shape->rounded = b.bf16;
+  p.direct = b.bf16 && b.dst != nullptr;
+  if (rc == HA_OK && p.direct) {
+    NsBatch d = b;
+    d.ld_x = b.cols;
+    d.plane_x = b.rows * b.cols;
+    rc = ns_map(&p.dst, reinterpret_cast<const __half*>(b.dst), d, 64, box);
+  }
   if (rc != HA_OK) return rc;
   cut_parts(coef, steps, &p.ends, &parts);
-  *out = parts & 1;
+  shape->out = p.direct ? -1 : parts & 1;
+  p.out = b.dst;
+  p.out_elems = b.n * b.rows * b.cols;
   p.tall = b.rows > b.cols;
   p.m = int(b.m);
   p.n = int(p.tall ? b.rows : b.cols);
