@@ -520,3 +520,43 @@ def test_training_loop():
             d = 1e-2 * 0.2 * math.sqrt(max(w.shape)) * definition(0.05 * g + 0.95 * m)
             err = float((params[i].double() - (w - d)).norm())
             assert err <= NS * float(d.norm()) + 2.0 ** -23 * float(w.norm())
+
+
+@pytest.mark.parametrize("budget", [1 << 32, 0], ids=["at_once", "one_by_one"])
+def test_many_shapes_in_one_step(monkeypatch, budget):
+    """More shapes than a run of the products takes, wide and tall, with sides up to 128 and beyond,
+    that end in parts of blocks, in one pass through the workspace and in many."""
+    import torch
+    from hybridagent_b200 import ZeroOneMuon
+    monkeypatch.setenv("HYBRIDAGENT_B200_MUON_BYTES", str(budget))
+    shapes = [(255, 257), (130, 700), (700, 131), (64, 1000), (257, 255), (129, 200), (513, 300), (300, 513), (150, 2000),
+              (255, 257), (20, 20), (641, 1300), (130, 700)]
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    params = [torch.nn.Parameter((torch.randn(s, generator=gen, device="cuda") * 0.02).bfloat16()) for s in shapes]
+    opt = ZeroOneMuon([{"params": params, "lr": 2e-2}], rank=0, world_size=1, weight_decay=0.01)
+    ref = Definition(opt, len(shapes), FACTORS["match_rms_adamw"])
+    for step in range(2):
+        set_grads(params, step, torch.bfloat16)
+        norm = opt.clip_grad_norm(1.0)
+        for i, p in enumerate(params):
+            ref.step(i, p, 1.0 / (norm + 1e-6) if norm > 1.0 else None)
+        opt.step()
+    for i, p in enumerate(params):
+        ref.check(i, opt, p, 2)
+
+
+@pytest.mark.parametrize("seed", range(4))
+def test_drawn_shapes(seed):
+    """Sizes next to the tiles' and blocks' edges, twice each: the same bits, and the definition's values."""
+    import random
+    import torch
+    from hybridagent_b200 import orthogonalize
+    rng = random.Random(seed)
+    edges = [1, 15, 16, 17, 31, 32, 33, 63, 64, 65, 127, 128, 129, 159, 160, 161, 191, 193, 255, 256, 257, 287, 289, 321, 383,
+             385, 449, 511, 513, 639, 641, 767, 769, 1023, 1025]
+    for _ in range(40):
+        rows, cols = rng.choice(edges), rng.choice(edges)
+        x = values("normal", (rng.choice([1, 2, 5]), rows, cols), torch.float32, seed=rows * 2000 + cols)
+        y = orthogonalize(x)
+        assert torch.equal(orthogonalize(x), y), (rows, cols)
+        assert off(y, definition(x)) <= NS_BF16, (rows, cols)
