@@ -104,21 +104,23 @@ class _Table:
         self.np = np.zeros(max(n, 1), dtype=dtype)
         nbytes = self.np.nbytes
         self.dev = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        self._bytes = self.np.view(np.uint8)
         self._ring = [torch.empty(nbytes, dtype=torch.uint8, pin_memory=True) for _ in range(self.RING)]
+        self._views = [buf.numpy() for buf in self._ring]
         self._events: list[torch.cuda.Event | None] = [None] * self.RING
         self._next = 0
 
     def upload(self) -> None:
         k = self._next
         self._next = (k + 1) % self.RING
-        if self._events[k] is not None:
-            self._events[k].synchronize()
-        buf = self._ring[k]
-        np.copyto(buf.numpy(), self.np.view(np.uint8))
-        self.dev.copy_(buf, non_blocking=True)
-        ev = torch.cuda.Event()
+        ev = self._events[k]
+        if ev is None:
+            ev = self._events[k] = torch.cuda.Event()
+        else:
+            ev.synchronize()
+        np.copyto(self._views[k], self._bytes)
+        self.dev.copy_(self._ring[k], non_blocking=True)
         ev.record()
-        self._events[k] = ev
 
     @property
     def ptr(self) -> int:
@@ -636,7 +638,7 @@ class ZeroOneAdamW:
 
     @staticmethod
     def _stream() -> int:
-        return torch.cuda.current_stream().cuda_stream
+        return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())  # of the current device, without objects
 
     def _owned_grads(self, c: _Class) -> tuple[list[torch.Tensor | None], np.ndarray]:
         grads, ptrs = [], np.zeros(len(c.owned), dtype=np.uint64)
