@@ -9,8 +9,8 @@
 // moves 10 bytes (G, M read, M written) and sums U's squares; the load kernel reads G and M again
 // (6 bytes; U itself is never stored, which would round it before its norm is known) and writes
 // the two fp16 planes of U / |U|; the weight kernel reads O and the master and writes the master and
-// the changed sectors of the copy.  A launch takes its tensors' descriptors as kernel parameters
-// (kSlice of them), so a step uploads no table and can be captured into a graph.
+// the changed sectors of the copy.  A launch takes its matrices' descriptors as kernel parameters
+// (kSlice of them, of any shapes), so a step uploads no table and can be captured into a graph.
 //
 // Sums: squares are taken and added in fp64 (gradients of 1e-30 or 1e25 keep their norm), each CTA
 // writes its own partial, and every reader adds a matrix's partials in the same order, so results
@@ -24,7 +24,7 @@
 namespace ha {
 namespace {
 
-constexpr int kSlice = 48;               // tensors of one launch: 48 x 64 bytes of kernel parameters
+constexpr int kSlice = 32;               // tensors of one launch: 32 x 120 bytes of kernel parameters
 constexpr int64_t kMinChunk = 8192;      // elements of one partial sum at least
 constexpr int64_t kMaxPartials = 512;    // partial sums of one matrix at most
 constexpr int kLoadChunk = kThreads * 8 * 4;  // padded elements of a CTA of the load and store kernels
@@ -34,8 +34,18 @@ constexpr int64_t kMaxPass = 4096;       // matrices of one pass
 constexpr int64_t kSliceBytes = 48 << 20;  // of matrices between the two reads of a slice: they stay in L2
 constexpr size_t kHeader = 256 + kMaxPass * 4;  // the workspace's error word, the matrices' counters
 
+// A matrix of a launch and its workspace; matrices of any shapes share launches.
+struct Entry {
+  ha_tensor t;
+  double* partials;
+  uint32_t* counter;
+  __half *hi, *lo;  // X's planes (weight kernel: hi holds the result)
+  uint32_t rows, cols, ld;
+  int32_t n_partials;
+  int64_t chunk;    // elements of a partial sum
+};
 struct Slice {
-  ha_tensor t[kSlice];
+  Entry e[kSlice];
 };
 
 struct MuonConst {
@@ -124,17 +134,19 @@ __global__ void __launch_bounds__(kThreads)
   if (threadIdx.x == 0) partials[int64_t(blockIdx.y) * gridDim.x + blockIdx.x] = acc;
 }
 
-// Momentum update and square sums of the direction.  Grid: (partials, tensors of the slice).
+// Momentum update and square sums of the direction.  Grid: (most partials of a matrix, matrices).
 template <int DT>
 __global__ void __launch_bounds__(kThreads)
-    momentum_kernel(const __grid_constant__ Slice s, MuonConst c, int64_t chunk, double* partials, uint32_t* error) {
+    momentum_kernel(const __grid_constant__ Slice s, MuonConst c, uint32_t* error) {
   __shared__ double red[kThreads / 32];
   using raw = typename Elem<DT>::raw;
   if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0 && error != nullptr) *error = 0;
-  const ha_tensor& t = s.t[blockIdx.y];
+  const Entry& entry = s.e[blockIdx.y];
+  if (int(blockIdx.x) >= entry.n_partials) return;
+  const ha_tensor& t = entry.t;
   const raw* grad = reinterpret_cast<const raw*>(t.grad);
   float* mom = reinterpret_cast<float*>(t.exp_avg);
-  const int64_t begin = int64_t(blockIdx.x) * chunk, end = min(begin + chunk, t.numel);
+  const int64_t begin = int64_t(blockIdx.x) * entry.chunk, end = min(begin + entry.chunk, t.numel);
   double acc = 0.0;
   auto one = [&](int64_t k) {
     float m = mom[k];
@@ -157,18 +169,28 @@ __global__ void __launch_bounds__(kThreads)
     for (int64_t k = begin + threadIdx.x; k < end; k += kThreads) one(k);
   }
   acc = block_sum_all(acc, red);
-  if (threadIdx.x == 0) partials[int64_t(blockIdx.y) * gridDim.x + blockIdx.x] = acc;
+  if (threadIdx.x == 0) entry.partials[blockIdx.x] = acc;
 }
 
 struct Shape {
   int64_t rows, cols, ld, plane;
 };
 
+// A matrix for the load kernel.
+struct Target {
+  const double* partials;
+  uint32_t* counter;
+  __half *hi, *lo;
+  uint32_t rows, cols, ld;
+  int n_partials;
+};
+
 // What the load kernel reads: element k of matrix `y` of the launch.
 template <int DT>
 struct PlainSource {
   const typename Elem<DT>::raw* x;
-  int64_t numel;
+  int64_t numel, plane;
+  Target first;
   struct View {
     const typename Elem<DT>::raw* x;
     __device__ bool aligned() const { return (reinterpret_cast<uintptr_t>(x) & 15) == 0; }
@@ -176,6 +198,14 @@ struct PlainSource {
     __device__ void eight(int64_t k, float (&v)[8]) const { load8<DT>(x + k, v); }
   };
   __device__ View view(int y) const { return View{x + y * numel}; }
+  __device__ Target target(int y) const {
+    Target t = first;
+    t.partials += int64_t(y) * t.n_partials;
+    t.counter += y;
+    t.hi += y * plane;
+    t.lo += y * plane;
+    return t;
+  }
 };
 template <int DT>
 struct MuonSource {
@@ -198,42 +228,43 @@ struct MuonSource {
     }
   };
   __device__ View view(int y) const {
-    return View{reinterpret_cast<const typename Elem<DT>::raw*>(s.t[y].grad),
-                reinterpret_cast<const float*>(s.t[y].exp_avg), c};
+    return View{reinterpret_cast<const typename Elem<DT>::raw*>(s.e[y].t.grad),
+                reinterpret_cast<const float*>(s.e[y].t.exp_avg), c};
+  }
+  __device__ Target target(int y) const {
+    const Entry& e = s.e[y];
+    return Target{e.partials, e.counter, e.hi, e.lo, e.rows, e.cols, e.ld, e.n_partials};
   }
 };
 
-// X0 = U / max(|U|_F, eps) into the high and low planes of matrix first + blockIdx.y (row padding
-// left alone).  Grid: (chunks of the padded matrix, matrices).
+// X0 = U / max(|U|_F, eps) into the matrices' high and low planes (row padding holds zeros).  Grid: (most
+// chunks of a padded matrix, matrices).
 template <class Source>
-__global__ void __launch_bounds__(kThreads) load_kernel(const __grid_constant__ Source src, Shape sh, int n_partials,
-                                                        const double* partials, double eps, int first, __half* hi,
-                                                        __half* lo, uint32_t* counter) {
-  if (blockIdx.x == 0 && threadIdx.x == 0) counter[first + blockIdx.y] = 0;
+__global__ void __launch_bounds__(kThreads) load_kernel(const __grid_constant__ Source src, double eps) {
   __shared__ double red[kThreads / 32];
-  const double* part = partials + int64_t(blockIdx.y) * n_partials;
+  const Target m = src.target(blockIdx.y);
+  const uint32_t per_row = m.ld >> 3;
+  const int64_t total = int64_t(m.rows) * per_row;
+  if (int64_t(blockIdx.x) * (kThreads * 4) >= total) return;
+  if (blockIdx.x == 0 && threadIdx.x == 0) *m.counter = 0;
   double sum = 0.0;
-  for (int i = threadIdx.x; i < n_partials; i += kThreads) sum += part[i];
+  for (int i = threadIdx.x; i < m.n_partials; i += kThreads) sum += m.partials[i];
   const double norm = sqrt(block_sum_all(sum, red));
   const float scale = float(double(kScaleX) / (norm < eps ? eps : norm));  // a NaN norm stays one
   const typename Source::View v = src.view(blockIdx.y);
-  hi += (first + int64_t(blockIdx.y)) * sh.plane;
-  lo += (first + int64_t(blockIdx.y)) * sh.plane;
-  const bool vec = v.aligned() && (sh.cols & 7) == 0;
-  const uint32_t per_row = uint32_t(sh.ld >> 3);
-  const int64_t total = sh.rows * per_row;
+  const bool vec = v.aligned() && (m.cols & 7) == 0;
 #pragma unroll
   for (int u = 0; u < 4; ++u) {
     const int64_t k = int64_t(blockIdx.x) * (kThreads * 4) + u * kThreads + threadIdx.x;
     if (k >= total) break;
     const uint32_t r = uint32_t(k) / per_row, c = (uint32_t(k) - r * per_row) * 8;
-    const int64_t e = int64_t(r) * sh.cols + c;
+    const int64_t e = int64_t(r) * m.cols + c;
     float x[8];
     if (vec) {
       v.eight(e, x);
     } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = c + i < sh.cols ? v.one(e + i) : 0.0f;
+      for (int i = 0; i < 8; ++i) x[i] = c + i < m.cols ? v.one(e + i) : 0.0f;
     }
     uint32_t h[4], l[4];
 #pragma unroll
@@ -245,9 +276,9 @@ __global__ void __launch_bounds__(kThreads) load_kernel(const __grid_constant__ 
       h[i] = *reinterpret_cast<const uint32_t*>(&p);
       l[i] = *reinterpret_cast<const uint32_t*>(&q);
     }
-    const int64_t at = int64_t(r) * sh.ld + c;
-    *reinterpret_cast<uint4*>(hi + at) = make_uint4(h[0], h[1], h[2], h[3]);
-    *reinterpret_cast<uint4*>(lo + at) = make_uint4(l[0], l[1], l[2], l[3]);
+    const int64_t at = int64_t(r) * m.ld + c;
+    *reinterpret_cast<uint4*>(m.hi + at) = make_uint4(h[0], h[1], h[2], h[3]);
+    *reinterpret_cast<uint4*>(m.lo + at) = make_uint4(l[0], l[1], l[2], l[3]);
   }
 }
 
@@ -307,8 +338,8 @@ __global__ void __launch_bounds__(kThreads)
 // factor and the plane's scale.  The stores follow adamw_kernel's (changed sectors only with DELTA).
 template <int DT, bool PEERS, bool DELTA>
 __global__ void __launch_bounds__(kThreads)
-    apply_kernel(const __grid_constant__ Slice s, const __half* x, Shape sh, int first, int use_decay, Peers peers,
-                 unsigned long long* changed, const uint32_t* error, uint32_t* status) {
+    apply_kernel(const __grid_constant__ Slice s, int use_decay, Peers peers, unsigned long long* changed,
+                 const uint32_t* error, uint32_t* status) {
   static_assert(!(DELTA && DT == HA_F32), "fp32 parameters are their own masters: always written");
   __shared__ uint32_t stored_in_cta;
   if (*error != 0) {  // a wait of the products ran out: the weights stay as they are
@@ -318,15 +349,18 @@ __global__ void __launch_bounds__(kThreads)
     }
     return;
   }
-  const ha_tensor& t = s.t[blockIdx.y];
-  x += (first + int64_t(blockIdx.y)) * sh.plane;
+  const Entry& entry = s.e[blockIdx.y];
+  const ha_tensor& t = entry.t;
+  if (int64_t(blockIdx.x) * kApplyChunk >= t.numel) return;
+  const __half* x = entry.hi;
+  const uint32_t cols = entry.cols, ld = entry.ld;
   float* master = reinterpret_cast<float*>(t.master);
   void* param = reinterpret_cast<void*>(t.param);
   const uint64_t pushed = DT == HA_F32 ? t.master : t.param;
   const float decay = t.decay, lr = __fmul_rn(t.neg_lr, 1.0f / kScaleX);
   const int64_t begin = int64_t(blockIdx.x) * kApplyChunk, end = min(begin + kApplyChunk, t.numel);
   const bool vec = (t.master & 15) == 0 && (DT == HA_F32 || (t.param & 7) == 0);
-  const bool vec_x = (sh.cols & 3) == 0;
+  const bool vec_x = (cols & 3) == 0;
   uint32_t stored = 0;
   if (DELTA && threadIdx.x == 0) stored_in_cta = 0;
   auto update = [&](float w, float o) {
@@ -334,12 +368,12 @@ __global__ void __launch_bounds__(kThreads)
     return __fmaf_rn(lr, o, w);
   };
   // Row and column of an element, 32-bit from the chunk's first one on (a chunk has 2^14 elements).
-  const int64_t row0 = begin / sh.cols;
-  const uint32_t col0 = uint32_t(begin - row0 * sh.cols), cols = uint32_t(sh.cols);
+  const int64_t row0 = begin / cols;
+  const uint32_t col0 = uint32_t(begin - row0 * cols);
   auto place = [&](int64_t k, uint32_t& c) {
     const uint32_t at = col0 + uint32_t(k - begin), r = at / cols;
     c = at - r * cols;
-    return x + (row0 + r) * sh.ld + c;
+    return x + (row0 + r) * ld + c;
   };
   auto one = [&](int64_t k) {
     uint32_t c;
@@ -379,7 +413,7 @@ __global__ void __launch_bounds__(kThreads)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               v[i] = __half2float(*o_at++);
-              if (++c == cols) c = 0, o_at += sh.ld - sh.cols;
+              if (++c == cols) c = 0, o_at += ld - cols;
             }
             o[u] = make_float4(v[0], v[1], v[2], v[3]);
           }
@@ -551,8 +585,10 @@ int orthogonalize(const void* src, void* dst, int64_t batch, int64_t rows, int64
       double* part = g.partials + k * g.n_partials;
       square_sum_kernel<DT><<<dim3(unsigned(g.n_partials), m), kThreads, 0, st>>>(
           x + k * numel, numel, g.chunk, part, i == 0 && k == 0 ? g.b.error : nullptr);
-      load_kernel<<<dim3(load_grid(g.b), m), kThreads, 0, st>>>(PlainSource<DT>{x + k * numel, numel}, sh, g.n_partials,
-                                                               part, ns.eps, int(k), g.b.hi[0], g.b.lo, g.b.counter);
+      const Target first{part, g.b.counter + k, g.b.hi[0] + k * sh.plane, g.b.lo + k * sh.plane, uint32_t(rows),
+                         uint32_t(cols), uint32_t(sh.ld), g.n_partials};
+      load_kernel<<<dim3(load_grid(g.b), m), kThreads, 0, st>>>(PlainSource<DT>{x + k * numel, numel, sh.plane, first},
+                                                               ns.eps);
     }
     // rows of 16-byte pieces: the last product stores the result itself
     uint16_t* out = static_cast<uint16_t*>(dst) + i * numel;
@@ -571,22 +607,21 @@ int orthogonalize(const void* src, void* dst, int64_t batch, int64_t rows, int64
 }
 
 template <int DT>
-void launch_apply(dim3 grid, cudaStream_t st, const Slice& s, const __half* x, const Shape& sh, int first,
-                  int use_decay, bool delta, const Peers& peers, unsigned long long* changed, const uint32_t* error,
-                  uint32_t* status) {
+void launch_apply(dim3 grid, cudaStream_t st, const Slice& s, int use_decay, bool delta, const Peers& peers,
+                  unsigned long long* changed, const uint32_t* error, uint32_t* status) {
   if constexpr (DT != HA_F32) {
     if (delta) {
       if (peers.n > 0)
-        apply_kernel<DT, true, true><<<grid, kThreads, 0, st>>>(s, x, sh, first, use_decay, peers, changed, error, status);
+        apply_kernel<DT, true, true><<<grid, kThreads, 0, st>>>(s, use_decay, peers, changed, error, status);
       else
-        apply_kernel<DT, false, true><<<grid, kThreads, 0, st>>>(s, x, sh, first, use_decay, peers, changed, error, status);
+        apply_kernel<DT, false, true><<<grid, kThreads, 0, st>>>(s, use_decay, peers, changed, error, status);
       return;
     }
   }
   if (peers.n > 0)
-    apply_kernel<DT, true, false><<<grid, kThreads, 0, st>>>(s, x, sh, first, use_decay, peers, changed, error, status);
+    apply_kernel<DT, true, false><<<grid, kThreads, 0, st>>>(s, use_decay, peers, changed, error, status);
   else
-    apply_kernel<DT, false, false><<<grid, kThreads, 0, st>>>(s, x, sh, first, use_decay, peers, changed, error, status);
+    apply_kernel<DT, false, false><<<grid, kThreads, 0, st>>>(s, use_decay, peers, changed, error, status);
 }
 
 template <int DT>
@@ -615,34 +650,56 @@ int muon_step(const ha_tensor* t, const int64_t* shape, int64_t n, const MuonCon
     }
     if (pass.groups == 0) continue;
     for (int stage = 0; stage < 2; ++stage) {  // momentum and load; then, after the products, the weights
+      MuonSource<DT> src;
+      src.c = c;
+      int m = 0;           // matrices of the launch
+      int64_t bytes_in = 0;
+      unsigned sums = 0, loads = 0, chunks = 0;
+      auto flush = [&]() {
+        if (m == 0) return HA_OK;
+        if (stage == 0) {
+          momentum_kernel<DT><<<dim3(sums, unsigned(m)), kThreads, 0, st>>>(src.s, c,
+                                                                           fresh ? pass.group[0].b.error : nullptr);
+          load_kernel<<<dim3(loads, unsigned(m)), kThreads, 0, st>>>(src, ns.eps);
+          fresh = false;
+        } else {
+          launch_apply<DT>(dim3(chunks, unsigned(m)), st, src.s, c.use_decay, delta, peers, changed, pass.group[0].b.error,
+                           status);
+        }
+        m = 0;
+        bytes_in = 0;
+        sums = loads = chunks = 0;
+        return check_launch(stage == 0 ? "ha_muon_step (momentum)" : "ha_muon_step (weights)");
+      };
       for (int i = 0; i < pass.groups; ++i) {
         const Group& g = pass.group[i];
-        const int64_t rows = g.b.rows, cols = g.b.cols;
-        const Shape sh{rows, cols, g.b.ld_x, g.b.plane_x};
-        MuonSource<DT> src;
-        src.c = c;
-        // momentum and load of a slice follow one another while it is in L2
-        int64_t slice = kSliceBytes / (rows * cols * (4 + int64_t(sizeof(typename Elem<DT>::raw))));
-        slice = stage != 0 || slice > kSlice ? kSlice : (slice < 1 ? 1 : slice);
-        for (int64_t k = g.begin, first = 0; first < g.b.n;) {
-          int m = 0;
-          for (; m < slice && first + m < g.b.n; ++k)
-            if (t[k].grad != 0) src.s.t[m++] = t[k];
-          if (stage == 0) {
-            double* part = g.partials + first * g.n_partials;
-            momentum_kernel<DT><<<dim3(unsigned(g.n_partials), unsigned(m)), kThreads, 0, st>>>(
-                src.s, c, g.chunk, part, fresh ? g.b.error : nullptr);
-            load_kernel<<<dim3(load_grid(g.b), unsigned(m)), kThreads, 0, st>>>(
-                src, sh, g.n_partials, part, ns.eps, int(first), g.b.hi[0], g.b.lo, g.b.counter);
-            fresh = false;
-          } else {
-            launch_apply<DT>(dim3(unsigned((rows * cols + kApplyChunk - 1) / kApplyChunk), unsigned(m)), st, src.s,
-                             g.b.hi[g.b.out], sh, int(first), c.use_decay, delta, peers, changed, g.b.error, status);
-          }
-          if (int rc = check_launch(stage == 0 ? "ha_muon_step (momentum)" : "ha_muon_step (weights)")) return rc;
-          first += m;
+        const int64_t numel = g.b.rows * g.b.cols;
+        const int64_t each = numel * (4 + int64_t(sizeof(typename Elem<DT>::raw)));
+        for (int64_t k = g.begin, z = 0; z < g.b.n; ++k) {
+          if (t[k].grad == 0) continue;
+          // full, or so much that the load kernel would no longer find it in L2
+          if (m == kSlice || (stage == 0 && m > 0 && bytes_in + each > kSliceBytes))
+            if (int rc = flush()) return rc;
+          Entry& e = src.s.e[m++];
+          e.t = t[k];
+          e.partials = g.partials + z * g.n_partials;
+          e.counter = g.b.counter + z;
+          e.hi = (stage == 0 ? g.b.hi[0] : g.b.hi[g.b.out]) + z * g.b.plane_x;
+          e.lo = g.b.lo + z * g.b.plane_x;
+          e.rows = uint32_t(g.b.rows);
+          e.cols = uint32_t(g.b.cols);
+          e.ld = uint32_t(g.b.ld_x);
+          e.n_partials = g.n_partials;
+          e.chunk = g.chunk;
+          bytes_in += each;
+          if (unsigned(g.n_partials) > sums) sums = unsigned(g.n_partials);
+          if (load_grid(g.b) > loads) loads = load_grid(g.b);
+          const unsigned w = unsigned((numel + kApplyChunk - 1) / kApplyChunk);
+          if (w > chunks) chunks = w;
+          ++z;
         }
       }
+      if (int rc = flush()) return rc;
       if (stage == 0)
         if (int rc = pass.run(ns, st)) return rc;
     }

@@ -186,9 +186,9 @@ class ZeroOneMuon(ZeroOneAdamW):
                   ctypes.byref(self._ns), int(changed_only), ctypes.byref(c.peers) if p2p else None,
                   c.changed_dev.data_ptr() if changed_only else None, self._muon_status.data_ptr(),
                   self._muon_ws.data_ptr(), self._muon_ws.numel(), self._stream())
-        # momentum, load and weights of each shape, and one run of the products: more where the workspace or a
-        # launch's parameters split them
-        self.launches += 3 * len({tuple(s) for s in c.shapes.tolist()}) + 1
+        # momentum, load and weights, and one run of the products: more where the workspace or a launch's
+        # parameters split them
+        self.launches += 4
 
     def state_summary(self) -> str:
         n = sum(len(c.layout.indices) for c in self._classes if c.muon)
