@@ -20,6 +20,7 @@
 #include "ha_common.cuh"
 #include "ha_param.cuh"
 #include "newton_schulz.cuh"
+#include "umma.cuh"
 
 namespace ha {
 namespace {
@@ -31,6 +32,10 @@ constexpr int kLoadChunk = kThreads * 8 * 4;  // padded elements of a CTA of the
 constexpr int64_t kApplyChunk = 16384;
 constexpr int kGroups = 4;               // 4-element groups per thread and pass of the weight kernel
 constexpr int64_t kMaxPass = 4096;       // matrices of one pass
+// Up to this size one CTA sums, updates and loads a matrix in one launch: 33 us against 37 for all of a
+// 64 x 96 matrix; at 131072 elements (48 of 256 x 512) one CTA for each costs 9 us more than two launches.
+constexpr int64_t kWholeElems = 32768;
+constexpr int kWholeThreads = 1024;
 constexpr int64_t kSliceBytes = 48 << 20;  // of matrices between the two reads of a slice: they stay in L2
 constexpr size_t kHeader = 256 + kMaxPass * 4;  // the workspace's error word, the matrices' counters
 
@@ -59,6 +64,7 @@ int64_t chunk_for(int64_t numel) {
   return (c + kMinChunk - 1) / kMinChunk * kMinChunk;
 }
 
+template <int THREADS = kThreads>
 __device__ __forceinline__ double block_sum_all(double x, double* smem) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
@@ -67,7 +73,7 @@ __device__ __forceinline__ double block_sum_all(double x, double* smem) {
   __syncthreads();
   x = 0.0;
 #pragma unroll
-  for (int w = 0; w < kThreads / 32; ++w) x += smem[w];
+  for (int w = 0; w < THREADS / 32; ++w) x += smem[w];
   return x;  // in every thread
 }
 
@@ -196,6 +202,9 @@ struct PlainSource {
     __device__ bool aligned() const { return (reinterpret_cast<uintptr_t>(x) & 15) == 0; }
     __device__ float one(int64_t k) const { return Elem<DT>::widen(x[k]); }
     __device__ void eight(int64_t k, float (&v)[8]) const { load8<DT>(x + k, v); }
+    // The first visit of an element (whole_kernel).
+    __device__ float first_one(int64_t k) const { return one(k); }
+    __device__ void first_eight(int64_t k, float (&v)[8]) const { eight(k, v); }
   };
   __device__ View view(int y) const { return View{x + y * numel}; }
   __device__ Target target(int y) const {
@@ -213,7 +222,7 @@ struct MuonSource {
   MuonConst c;
   struct View {
     const typename Elem<DT>::raw* g;
-    const float* m;
+    float* m;
     MuonConst c;
     __device__ bool aligned() const {
       return ((reinterpret_cast<uintptr_t>(g) | reinterpret_cast<uintptr_t>(m)) & 15) == 0;
@@ -226,10 +235,26 @@ struct MuonSource {
 #pragma unroll
       for (int i = 0; i < 8; ++i) v[i] = direction_elem<DT>(c, a[i], v[i]);
     }
+    // The first visit updates the momentum.
+    __device__ float first_one(int64_t k) const {
+      float w = m[k];
+      const float u = momentum_elem<DT>(c, Elem<DT>::widen(g[k]), w);
+      m[k] = w;
+      return u;
+    }
+    __device__ void first_eight(int64_t k, float (&v)[8]) const {
+      float a[8], w[8];
+      load8<DT>(g + k, a);
+      load8<HA_F32>(m + k, w);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = momentum_elem<DT>(c, a[i], w[i]);
+      reinterpret_cast<float4*>(m + k)[0] = make_float4(w[0], w[1], w[2], w[3]);
+      reinterpret_cast<float4*>(m + k)[1] = make_float4(w[4], w[5], w[6], w[7]);
+    }
   };
   __device__ View view(int y) const {
     return View{reinterpret_cast<const typename Elem<DT>::raw*>(s.e[y].t.grad),
-                reinterpret_cast<const float*>(s.e[y].t.exp_avg), c};
+                reinterpret_cast<float*>(s.e[y].t.exp_avg), c};
   }
   __device__ Target target(int y) const {
     const Entry& e = s.e[y];
@@ -237,11 +262,44 @@ struct MuonSource {
   }
 };
 
-// X0 = U / max(|U|_F, eps) into the matrices' high and low planes (row padding holds zeros).  Grid: (most
-// chunks of a padded matrix, matrices).
+// Eight padded elements of a matrix, X0 = U / max(|U|_F, eps), into its high and low planes (row padding
+// holds zeros).
+template <class View>
+__device__ __forceinline__ void load_group(const Target& m, const View& v, bool vec, float scale, uint32_t per_row,
+                                           int64_t k) {
+  const uint32_t r = uint32_t(k) / per_row, c = (uint32_t(k) - r * per_row) * 8;
+  const int64_t e = int64_t(r) * m.cols + c;
+  float x[8];
+  if (vec) {
+    v.eight(e, x);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = c + i < m.cols ? v.one(e + i) : 0.0f;
+  }
+  uint32_t h[4], l[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float a = __fmul_rn(x[2 * i], scale), b = __fmul_rn(x[2 * i + 1], scale);
+    const __half2 p = __floats2half2_rn(a, b);
+    const float2 f = __half22float2(p);
+    const __half2 q = __floats2half2_rn((a - f.x) * kScaleLo, (b - f.y) * kScaleLo);
+    h[i] = *reinterpret_cast<const uint32_t*>(&p);
+    l[i] = *reinterpret_cast<const uint32_t*>(&q);
+  }
+  const int64_t at = int64_t(r) * m.ld + c;
+  *reinterpret_cast<uint4*>(m.hi + at) = make_uint4(h[0], h[1], h[2], h[3]);
+  *reinterpret_cast<uint4*>(m.lo + at) = make_uint4(l[0], l[1], l[2], l[3]);
+}
+__device__ __forceinline__ float scale_of(double sum, double eps) {
+  const double norm = sqrt(sum);
+  return float(double(kScaleX) / (norm < eps ? eps : norm));  // a NaN norm stays one
+}
+
+// Grid: (most chunks of a padded matrix, matrices); the square sums are there.
 template <class Source>
 __global__ void __launch_bounds__(kThreads) load_kernel(const __grid_constant__ Source src, double eps) {
   __shared__ double red[kThreads / 32];
+  grid_launch_dependents();
   const Target m = src.target(blockIdx.y);
   const uint32_t per_row = m.ld >> 3;
   const int64_t total = int64_t(m.rows) * per_row;
@@ -249,37 +307,49 @@ __global__ void __launch_bounds__(kThreads) load_kernel(const __grid_constant__ 
   if (blockIdx.x == 0 && threadIdx.x == 0) *m.counter = 0;
   double sum = 0.0;
   for (int i = threadIdx.x; i < m.n_partials; i += kThreads) sum += m.partials[i];
-  const double norm = sqrt(block_sum_all(sum, red));
-  const float scale = float(double(kScaleX) / (norm < eps ? eps : norm));  // a NaN norm stays one
+  const float scale = scale_of(block_sum_all(sum, red), eps);
   const typename Source::View v = src.view(blockIdx.y);
   const bool vec = v.aligned() && (m.cols & 7) == 0;
 #pragma unroll
   for (int u = 0; u < 4; ++u) {
     const int64_t k = int64_t(blockIdx.x) * (kThreads * 4) + u * kThreads + threadIdx.x;
-    if (k >= total) break;
-    const uint32_t r = uint32_t(k) / per_row, c = (uint32_t(k) - r * per_row) * 8;
-    const int64_t e = int64_t(r) * m.cols + c;
-    float x[8];
-    if (vec) {
-      v.eight(e, x);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = c + i < m.cols ? v.one(e + i) : 0.0f;
-    }
-    uint32_t h[4], l[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float a = __fmul_rn(x[2 * i], scale), b = __fmul_rn(x[2 * i + 1], scale);
-      const __half2 p = __floats2half2_rn(a, b);
-      const float2 f = __half22float2(p);
-      const __half2 q = __floats2half2_rn((a - f.x) * kScaleLo, (b - f.y) * kScaleLo);
-      h[i] = *reinterpret_cast<const uint32_t*>(&p);
-      l[i] = *reinterpret_cast<const uint32_t*>(&q);
-    }
-    const int64_t at = int64_t(r) * m.ld + c;
-    *reinterpret_cast<uint4*>(m.hi + at) = make_uint4(h[0], h[1], h[2], h[3]);
-    *reinterpret_cast<uint4*>(m.lo + at) = make_uint4(l[0], l[1], l[2], l[3]);
+    if (k < total) load_group(m, v, vec, scale, per_row, k);
   }
+}
+
+// The same for matrices of at most kWholeElems elements, a CTA each, square sums and momentum included.
+template <class Source>
+__global__ void __launch_bounds__(kWholeThreads)
+    whole_kernel(const __grid_constant__ Source src, double eps, uint32_t* error) {
+  __shared__ double red[kWholeThreads / 32];
+  grid_launch_dependents();
+  const Target m = src.target(blockIdx.x);
+  const typename Source::View v = src.view(blockIdx.x);
+  if (threadIdx.x == 0) {
+    *m.counter = 0;
+    if (blockIdx.x == 0 && error != nullptr) *error = 0;
+  }
+  const int numel = int(m.rows * m.cols);
+  const bool flat = v.aligned();
+  double acc = 0.0;
+  if (flat) {
+    for (int k = threadIdx.x * 8; k < numel; k += kWholeThreads * 8) {
+      if (k + 8 <= numel) {
+        float x[8];
+        v.first_eight(k, x);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) add_square(acc, x[i]);
+      } else {
+        for (int i = k; i < numel; ++i) add_square(acc, v.first_one(i));
+      }
+    }
+  } else {
+    for (int k = threadIdx.x; k < numel; k += kWholeThreads) add_square(acc, v.first_one(k));
+  }
+  const float scale = scale_of(block_sum_all<kWholeThreads>(acc, red), eps);  // (and a barrier: momenta are written)
+  const uint32_t per_row = m.ld >> 3;
+  const int total = int(m.rows * per_row);
+  for (int k = threadIdx.x; k < total; k += kWholeThreads) load_group(m, v, flat && (m.cols & 7) == 0, scale, per_row, k);
 }
 
 // The orthogonalised matrices as bf16 (`rounded`: which they are; NaN if a wait of the products ran out), eight
@@ -583,12 +653,16 @@ int orthogonalize(const void* src, void* dst, int64_t batch, int64_t rows, int64
     for (int64_t k = 0; k < n; k += slice) {
       const unsigned m = unsigned(n - k < slice ? n - k : slice);
       double* part = g.partials + k * g.n_partials;
-      square_sum_kernel<DT><<<dim3(unsigned(g.n_partials), m), kThreads, 0, st>>>(
-          x + k * numel, numel, g.chunk, part, i == 0 && k == 0 ? g.b.error : nullptr);
       const Target first{part, g.b.counter + k, g.b.hi[0] + k * sh.plane, g.b.lo + k * sh.plane, uint32_t(rows),
                          uint32_t(cols), uint32_t(sh.ld), g.n_partials};
-      load_kernel<<<dim3(load_grid(g.b), m), kThreads, 0, st>>>(PlainSource<DT>{x + k * numel, numel, sh.plane, first},
-                                                               ns.eps);
+      const PlainSource<DT> source{x + k * numel, numel, sh.plane, first};
+      if (numel <= kWholeElems) {
+        whole_kernel<<<m, kWholeThreads, 0, st>>>(source, ns.eps, i == 0 && k == 0 ? g.b.error : nullptr);
+        continue;
+      }
+      square_sum_kernel<DT><<<dim3(unsigned(g.n_partials), m), kThreads, 0, st>>>(
+          x + k * numel, numel, g.chunk, part, i == 0 && k == 0 ? g.b.error : nullptr);
+      load_kernel<<<dim3(load_grid(g.b), m), kThreads, 0, st>>>(source, ns.eps);
     }
     // rows of 16-byte pieces: the last product stores the result itself
     uint16_t* out = static_cast<uint16_t*>(dst) + i * numel;
@@ -650,25 +724,30 @@ int muon_step(const ha_tensor* t, const int64_t* shape, int64_t n, const MuonCon
     }
     if (pass.groups == 0) continue;
     for (int stage = 0; stage < 2; ++stage) {  // momentum and load; then, after the products, the weights
-      MuonSource<DT> src;
-      src.c = c;
-      int m = 0;           // matrices of the launch
-      int64_t bytes_in = 0;
-      unsigned sums = 0, loads = 0, chunks = 0;
-      auto flush = [&]() {
-        if (m == 0) return HA_OK;
-        if (stage == 0) {
-          momentum_kernel<DT><<<dim3(sums, unsigned(m)), kThreads, 0, st>>>(src.s, c,
-                                                                           fresh ? pass.group[0].b.error : nullptr);
-          load_kernel<<<dim3(loads, unsigned(m)), kThreads, 0, st>>>(src, ns.eps);
+      struct Batch {
+        MuonSource<DT> src;
+        int m = 0;  // matrices of the launch
+        int64_t bytes = 0;
+        unsigned sums = 0, loads = 0, chunks = 0;
+      } large, small;
+      large.src.c = small.src.c = c;
+      auto flush = [&](Batch& b) {
+        if (b.m == 0) return HA_OK;
+        uint32_t* error = fresh ? pass.group[0].b.error : nullptr;
+        if (stage == 1) {
+          launch_apply<DT>(dim3(b.chunks, unsigned(b.m)), st, b.src.s, c.use_decay, delta, peers, changed,
+                           pass.group[0].b.error, status);
+        } else if (&b == &small) {
+          whole_kernel<<<unsigned(b.m), kWholeThreads, 0, st>>>(b.src, ns.eps, error);
           fresh = false;
         } else {
-          launch_apply<DT>(dim3(chunks, unsigned(m)), st, src.s, c.use_decay, delta, peers, changed, pass.group[0].b.error,
-                           status);
+          momentum_kernel<DT><<<dim3(b.sums, unsigned(b.m)), kThreads, 0, st>>>(b.src.s, c, error);
+          load_kernel<<<dim3(b.loads, unsigned(b.m)), kThreads, 0, st>>>(b.src, ns.eps);
+          fresh = false;
         }
-        m = 0;
-        bytes_in = 0;
-        sums = loads = chunks = 0;
+        b.m = 0;
+        b.bytes = 0;
+        b.sums = b.loads = b.chunks = 0;
         return check_launch(stage == 0 ? "ha_muon_step (momentum)" : "ha_muon_step (weights)");
       };
       for (int i = 0; i < pass.groups; ++i) {
@@ -677,10 +756,11 @@ int muon_step(const ha_tensor* t, const int64_t* shape, int64_t n, const MuonCon
         const int64_t each = numel * (4 + int64_t(sizeof(typename Elem<DT>::raw)));
         for (int64_t k = g.begin, z = 0; z < g.b.n; ++k) {
           if (t[k].grad == 0) continue;
+          Batch& b = stage == 0 && numel <= kWholeElems ? small : large;
           // full, or so much that the load kernel would no longer find it in L2
-          if (m == kSlice || (stage == 0 && m > 0 && bytes_in + each > kSliceBytes))
-            if (int rc = flush()) return rc;
-          Entry& e = src.s.e[m++];
+          if (b.m == kSlice || (stage == 0 && b.m > 0 && b.bytes + each > kSliceBytes))
+            if (int rc = flush(b)) return rc;
+          Entry& e = b.src.s.e[b.m++];
           e.t = t[k];
           e.partials = g.partials + z * g.n_partials;
           e.counter = g.b.counter + z;
@@ -691,15 +771,16 @@ int muon_step(const ha_tensor* t, const int64_t* shape, int64_t n, const MuonCon
           e.ld = uint32_t(g.b.ld_x);
           e.n_partials = g.n_partials;
           e.chunk = g.chunk;
-          bytes_in += each;
-          if (unsigned(g.n_partials) > sums) sums = unsigned(g.n_partials);
-          if (load_grid(g.b) > loads) loads = load_grid(g.b);
+          b.bytes += each;
+          if (unsigned(g.n_partials) > b.sums) b.sums = unsigned(g.n_partials);
+          if (load_grid(g.b) > b.loads) b.loads = load_grid(g.b);
           const unsigned w = unsigned((numel + kApplyChunk - 1) / kApplyChunk);
-          if (w > chunks) chunks = w;
+          if (w > b.chunks) b.chunks = w;
           ++z;
         }
       }
-      if (int rc = flush()) return rc;
+      if (int rc = flush(large)) return rc;
+      if (int rc = flush(small)) return rc;
       if (stage == 0)
         if (int rc = pass.run(ns, st)) return rc;
     }

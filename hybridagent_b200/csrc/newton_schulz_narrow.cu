@@ -132,6 +132,7 @@ __global__ void __launch_bounds__(kThreadsN, 1) narrow_kernel(const __grid_const
   tc_fence_before();
   cluster_sync();
   tc_fence_after();
+  grid_wait();  // the load kernel's planes
   const uint32_t tmem = tmem_s, lanes = tmem + (uint32_t(quarter * 32) << 16);
   uint32_t done_phase = 0;  // bit i: phase of bars.done[i]
   auto wait_done = [&](int i) {
@@ -544,13 +545,15 @@ int narrow_run(NsBatch* shape, const float* coef, int steps, int sms, cudaStream
   cfg.blockDim = dim3(kThreadsN);
   cfg.dynamicSmemBytes = kSmemN;
   cfg.stream = st;
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = unsigned(p.cluster);
-  attr.val.clusterDim.y = 1;
-  attr.val.clusterDim.z = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = unsigned(p.cluster);
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, narrow_kernel, p);
   if (e != cudaSuccess) {
     cudaGetLastError();
