@@ -700,8 +700,15 @@ int make_stages(NsBatch* shape, const float* coef, int steps, int map0, int coun
   return count;
 }
 
-// Cuts a shape's stages into tiles; adds its work, in 128 x 128 x 64 products of a CTA, to *work, and the
-// work of the busiest CTA, if the shape ran alone, to *alone.  False if there are too many tiles.
+// Cuts a shape's stages into tiles; adds its share of the chip's time, in cycles, to *work, and the time
+// that it would take alone to *alone.  False if there are too many tiles.
+//
+// The tile is 256 x 256 on a CTA pair or 128 x 128 on one CTA.  The large one reads half the operand bytes per product:
+// measured, 64 of K take 600 cycles of a pair's tile and 500 of the small one, a quarter of it, which waits
+// for its operands.  But a stage of large tiles takes 16 thousand cycles from its first load to its last counter
+// beside that, of small ones 8 thousand, unless there are tiles to fill the wait, and few large tiles leave
+// SMs idle: small / large in us, 16 x 512 x 512: 122 / 157; 1 x 2048 x 2048: 218 / 265; 19 x 1152 x 1600:
+// 1181 / 1006; 13 x 1920 x 1536: 1514 / 1129.
 bool cut(Stage* stages, int count, int64_t batch, int cg, int workers, double* work, double* alone) {
   const int tile = 128 * cg;
   uint32_t before = 0;
@@ -715,9 +722,10 @@ bool cut(Stage* stages, int count, int64_t batch, int cg, int workers, double* w
     g.m_fast = g.tiles_m <= g.tiles_n;  // the shorter side first: its operand panels stay in L2
     g.before = before;
     before += uint32_t(per) * 2 * cg;   // both store warps of each of its CTAs
-    const double each = double(cg) * ((g.K + kBK - 1) / kBK);
-    *work += each * double(per * batch) / workers;
-    *alone += each * double((per * batch + workers - 1) / workers);
+    const double tiles = double(per * batch), each = (cg == 1 ? 500.0 : 600.0) * ((g.K + kBK - 1) / kBK);
+    const double wait = cg == 1 ? 8e3 : 16e3;
+    *work += each * tiles / workers;
+    *alone += each * double((per * batch + workers - 1) / workers) + (tiles > workers ? wait * workers / tiles : wait);
   }
   return true;
 }
@@ -766,9 +774,7 @@ int launch(const Args& p, int sms, cudaStream_t st) {
   return HA_OK;
 }
 
-// One launch for `n` shapes.  The tile: 256 x 256 on a CTA pair reads half the operand bytes per product of a
-// 128 x 128 tile on one CTA and runs 1.35 times as fast where both fill the chip (2.75 against 3.70 ms for five
-// steps of 4096 x 12288), but leaves SMs idle when there are few tiles and pads more.
+// One launch for `n` shapes.
 template <class Args>
 int run(NsBatch** shapes, int n, const float* coef, int steps, int sms, cudaStream_t st) {
   constexpr int kRoom = int(sizeof(Args::job) / sizeof(Job));
@@ -791,7 +797,7 @@ int run(NsBatch** shapes, int n, const float* coef, int steps, int sms, cudaStre
   };
   const double two = cost(2), one = cost(1);
   if (one < 0) return fail(HA_ERR_INVALID, "Newton-Schulz products with too many tiles");
-  const int cg = 1.35 * one <= two ? 1 : 2;
+  const int cg = two < 0 || one <= two ? 1 : 2;
   if (cg == 2) cost(2);
   int jobs = 0;
   for (int i = 0; i < n; ++i)
