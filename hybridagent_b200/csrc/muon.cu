@@ -30,7 +30,8 @@ constexpr int64_t kMinChunk = 8192;      // elements of one partial sum at least
 constexpr int64_t kMaxPartials = 512;    // partial sums of one matrix at most
 constexpr int kLoadChunk = kThreads * 8 * 4;  // padded elements of a CTA of the load and store kernels
 constexpr int64_t kApplyChunk = 16384;
-constexpr int kGroups = 4;               // 4-element groups per thread and pass of the weight kernel
+constexpr int kGroups = 2;               // 4-element groups per thread and pass of the weight kernel (361 us for 193 M bf16 weights, at HBM's rate;
+                                         // 4: 475, 8: 598: fewer CTAs fit an SM)
 constexpr int64_t kMaxPass = 4096;       // matrices of one pass
 // Up to this size one CTA sums, updates and loads a matrix in one launch: 33 us against 37 for all of a
 // 64 x 96 matrix; at 131072 elements (48 of 256 x 512) one CTA for each costs 9 us more than two launches.
