@@ -22,12 +22,12 @@
 // 3 m^2 n + 5 m^3.  See pairs() for where that is done and what it costs in accuracy.
 //
 // All products of all steps of all shapes run in one persistent launch, one CTA per SM, one or two CTAs to a
-// tile: a step of a small matrix takes a few microseconds, less than what three launches cost.  The work is a list
-// of jobs (a stage, that is one product, of some matrices of one shape), whose tiles the CTAs take in turn; a tile
+// tile: a step of a small matrix takes a few microseconds, less than what three launches cost.  The work is a list of
+// jobs (a stage, that is one product, of all matrices of one shape), whose tiles the CTAs take in turn; a tile
 // waits until all tiles of the previous stage of its matrix are stored (a counter per matrix in global memory), so
 // matrices need not wait for one another and a job's last tiles run beside the next one's first.  Jobs of several
-// shapes alternate, so that one shape's tiles fill the time in which another's results travel.  A job waits only for jobs before it
-// in the list, and the launch is cooperative: all CTAs are resident, so the waits end.
+// shapes alternate, so that one shape's tiles fill the time in which another's results travel.  A job waits only for
+// jobs before it in the list, and the launch is cooperative: all CTAs are resident, so the waits end.
 //
 // In a CTA, warp 0 feeds a ring of 128-byte-swizzled operand tiles by TMA, one thread of warp 1 issues the
 // MMAs, and eight epilogue warps read the accumulators from one of two TMEM buffers while the next tile
@@ -37,6 +37,12 @@
 // matrix's counter after its last block of a tile.  Fetching, storing and signalling take long, so none is left
 // to the epilogue warps: products with small K are bound by the epilogue.  Tall matrices (rows > cols) are not
 // transposed: both operand layouts (K contiguous, or M/N contiguous) are read by the MMA as they lie.
+//
+// Measured, from call to result: 4096 x 4096 1.26 ms and 4096 x 12288 2.32 ms, 1.1 PFLOP/s executed (symmetric tiles
+// once), where the chip's power holds large fp16 products at 1.26 to 1.31; two of 17408 x 5120 10.3 ms; 128 of
+// 704 x 2816 3.9 ms, bound by the traffic of X's planes, 0.51 GB each, and by 704 in tiles of 256; 48 of 256 x 512
+// 115 us and 8 of 1024 x 256 100 us, bound by the way from one stage to the next (load, products, epilogue, store,
+// counter: 4 to 8 us).
 #include <cuda.h>
 
 #include <algorithm>
@@ -91,9 +97,9 @@ struct Stage {
   uint8_t map_a, map_b, map_out, map_2, map_add;
   int8_t epilogue, m_fast, a_mn, b_mn, keep_low;  // *_mn: the operand's M / N index is the contiguous one
 };
-// A stage of `count` matrices from `first` on.
+// A stage of all `count` matrices of its shape.
 struct Job {
-  uint16_t stage, first, count, reserved;
+  uint16_t stage, count;
 };
 
 // Kernel parameters; small ones launch faster.
@@ -126,11 +132,10 @@ struct TileAt {
   int z, i, j;  // matrix, tile row, tile column
 };
 // Tile `t` of a job.  Symmetric stages: the tiles on and below the diagonal, row by row.
-__device__ __forceinline__ TileAt tile_at(const Stage& g, const Job& job, int t) {
+__device__ __forceinline__ TileAt tile_at(const Stage& g, int t) {
   TileAt a;
   a.z = t / g.per_matrix;
   const int r = t - a.z * g.per_matrix;
-  a.z += job.first;
   if (g.epilogue <= kPoly) {
     int i = int((sqrtf(8.0f * float(r) + 1.0f) - 1.0f) * 0.5f);
     while (i * (i + 1) / 2 > r) --i;
@@ -192,7 +197,7 @@ __device__ __forceinline__ bool epilogue(const Stage& g, const Job& job, Warp& w
   const float scale = g.scale, add_scale = g.add, diag = g.diag;
   const int tiles = job.count * g.per_matrix;
   for (int t = w.walk.start(); t < tiles; t += w.walk.step) {
-    const TileAt at = tile_at(g, job, t);
+    const TileAt at = tile_at(g, t);
     const int blocks = blocks_of<CG>(g, at, w.rank);
     const int row = at.i * kTile + w.rank * kBM + mine;
     if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&sh.acc_full[w.acc]), w.acc_phase, &sh.stop))) return false;
@@ -294,7 +299,7 @@ __device__ __forceinline__ void feed_blocks(const Args& p, Shared& sh, uint32_t 
     const int tiles = job.count * g.per_matrix;
     for (int t = walk.start(); t < tiles; t += walk.step) {
       ++tile;
-      const TileAt at = tile_at(g, job, t);
+      const TileAt at = tile_at(g, t);
       const int blocks = blocks_of<CG>(g, at, rank);
       for (int k = 0; k < blocks; ++k, ++n) {
         const uint32_t b = n % kBlocks, full = smem_u32(&sh.blk_full[b]);
@@ -324,7 +329,7 @@ __device__ __forceinline__ void store_blocks(const Args& p, Shared& sh, uint32_t
     const int tiles = job.count * g.per_matrix;
     for (int t = walk.start(); t < tiles; t += walk.step) {
       ++tile;
-      const TileAt at = tile_at(g, job, t);
+      const TileAt at = tile_at(g, t);
       const int blocks = blocks_of<CG>(g, at, rank), row = at.i * (128 * CG) + rank * kBM;
       uint32_t last = kBlocks;  // block of the store before, not yet handed back
       for (int k = int((n ^ group) & 1); k < blocks; k += 2) {
@@ -414,7 +419,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) newton_schulz_kernel(const __
         const bool a_mn = g.a_mn, b_mn = g.b_mn;
         int ready = -1;
         for (int t = walk.start(); t < tiles && ok; t += walk.step) {
-          const TileAt at = tile_at(g, job, t);
+          const TileAt at = tile_at(g, t);
           if (at.z != ready) {
             ok = counter_wait(p.counter + g.counter + at.z, g.before, &sh.stop);
             if (!ok) break;
@@ -565,7 +570,8 @@ int make_map(CUtensorMap* map, const Operand& x, int64_t n, int box_cols, int bo
   const cuuint32_t box[3] = {cuuint32_t(box_cols), cuuint32_t(box_rows), 1};
   const cuuint32_t step[3] = {1, 1, 1};
   const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<__half*>(x.base), dims, strides, box, step,
-                        CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS)
     return fail(HA_ERR_CUDA, "cuTensorMapEncodeTiled: error %d for %lld x %lld x %lld", int(r), (long long)n,
                 (long long)x.rows, (long long)x.cols);
@@ -741,7 +747,7 @@ int place(const Stage* stages, int first_stage, int count, const NsBatch& b, Pla
   auto cost = [&](int s) { return double(stages[s].per_matrix) * ((stages[s].K + kBK - 1) / kBK); };
   for (int s = 0; s < count; ++s) total += cost(s);
   for (int s = 0; s < count; ++s) {
-    out[n++] = Placed{Job{uint16_t(first_stage + s), 0, uint16_t(b.n), 0}, done / total};
+    out[n++] = Placed{Job{uint16_t(first_stage + s), uint16_t(b.n)}, done / total};
     done += cost(s);
   }
   return n;
@@ -783,8 +789,8 @@ int run(NsBatch** shapes, int n, const float* coef, int steps, int sms, cudaStre
   int first[kManyShapes + 1] = {0};
   for (int i = 0; i < n; ++i) {
     if (int rc = make_maps(*shapes[i], p.map + i * kMaps)) return rc;
-    first[i + 1] = first[i] + make_stages(shapes[i], coef, steps, i * kMaps, int(shapes[i]->counter - shapes[0]->counter),
-                                          p.stage + first[i]);
+    const int counter = int(shapes[i]->counter - shapes[0]->counter);
+    first[i + 1] = first[i] + make_stages(shapes[i], coef, steps, i * kMaps, counter, p.stage + first[i]);
   }
   auto cost = [&](int cg) {
     double work = 0.0, longest = 0.0;

@@ -72,7 +72,9 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
 
 // Programmatic dependent launch: lets the next kernel of the stream, if it was launched for that, start its
 // prologue; and waits there until the kernels before have finished and their writes are visible.
-__device__ __forceinline__ void grid_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void grid_launch_dependents() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
 __device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 // Bounded wait: false once `kWaitNs` have passed, or as soon as another thread of the CTA gave up

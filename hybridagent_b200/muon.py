@@ -25,6 +25,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import operator
 import os
 
 import numpy as np
@@ -39,11 +40,12 @@ ADJUST_LR = ("match_rms_adamw", "original", None)
 
 def _ns_params(steps: int, coefficients, eps: float) -> _lib.NsParams:
     """``coefficients``: one (a, b, c) for every step, or one for each."""
-    steps = int(steps)
+    steps = operator.index(steps)
     if not 1 <= steps <= _lib.HA_NS_MAX_STEPS:
         raise ValueError(f"steps must be between 1 and {_lib.HA_NS_MAX_STEPS}")
-    rows = [tuple(float(v) for v in row) for row in
-            (coefficients if hasattr(coefficients[0], "__len__") else [coefficients] * steps)]
+    coefficients = list(coefficients)
+    each = bool(coefficients) and hasattr(coefficients[0], "__len__")
+    rows = [tuple(float(v) for v in row) for row in (coefficients if each else [coefficients] * steps)]
     if len(rows) != steps or any(len(row) != 3 for row in rows):
         raise ValueError("coefficients must be (a, b, c), or one (a, b, c) for each step")
     out = _lib.NsParams()
@@ -176,9 +178,7 @@ class ZeroOneMuon(ZeroOneAdamW):
 
     def _update_muon(self, c, sc: _lib.AdamwScalars, changed_only: bool, p2p: bool) -> None:
         """The Muon update of class c's owned matrices that have a gradient."""
-        if int(self._muon_status[0]) != 0:
-            raise RuntimeError("Muon step: a wait inside the Newton-Schulz products ran out; the matrices of that "
-                               "step were not updated")
+        self._check_status()
         ms = _lib.MuonScalars(np.float32(self.momentum), np.float32(1.0 - self.momentum), int(self.nesterov),
                               sc.use_decay, sc.clip, sc.clip_mult)
         table = np.ascontiguousarray(c.table.np[c.order])
@@ -189,6 +189,17 @@ class ZeroOneMuon(ZeroOneAdamW):
         # momentum, load and weights, and one run of the products: more where the workspace or a launch's
         # parameters split them
         self.launches += 4
+
+    def _check_status(self) -> None:
+        """Raises if the products of a step that has run gave up."""
+        if int(self._muon_status[0]) != 0:
+            raise RuntimeError("Muon step: a wait inside the Newton-Schulz products ran out; the matrices of that "
+                               "step were not updated")
+
+    def state_dict(self) -> dict:
+        state = super().state_dict()  # (waits for the steps before)
+        self._check_status()
+        return state
 
     def state_summary(self) -> str:
         n = sum(len(c.layout.indices) for c in self._classes if c.muon)

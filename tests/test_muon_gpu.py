@@ -518,7 +518,7 @@ def test_training_loop():
             g = params[i].grad.double()
             m = 0.95 * m + 0.05 * g
             d = 1e-2 * 0.2 * math.sqrt(max(w.shape)) * definition(0.05 * g + 0.95 * m)
-            err = float((params[i].double() - (w - d)).norm())
+            err = float((params[i].detach().double() - (w - d)).norm())
             assert err <= NS * float(d.norm()) + 2.0 ** -23 * float(w.norm())
 
 
@@ -560,3 +560,19 @@ def test_drawn_shapes(seed):
         y = orthogonalize(x)
         assert torch.equal(orthogonalize(x), y), (rows, cols)
         assert off(y, definition(x)) <= NS_BF16, (rows, cols)
+
+
+def test_a_step_that_gave_up_is_reported():
+    """What the weight kernel writes when a wait of the products ran out, here written by the host."""
+    import torch
+    params, opt, _ = build("small", torch.bfloat16)
+    set_grads(params, 0, torch.bfloat16)
+    opt.clip_grad_norm(1.0)
+    opt.step()
+    opt.state_dict()
+    opt._muon_status[0] = 1
+    with pytest.raises(RuntimeError, match="ran out"):
+        opt.state_dict()
+    set_grads(params, 1, torch.bfloat16)
+    with pytest.raises(RuntimeError, match="ran out"):
+        opt.step()

@@ -133,7 +133,7 @@ def test_python_arguments():
         orthogonalize(torch.zeros(5))
     for kw, message in ((dict(steps=0), "steps"), (dict(steps=17), "steps"), (dict(coefficients=(1.0, 2.0)), "coefficients"),
                         (dict(coefficients=[(1.5, -0.5, 0.0)] * 4), "coefficients"),
-                        (dict(coefficients=[(1.5, -0.5)] * 5), "coefficients")):
+                        (dict(coefficients=[(1.5, -0.5)] * 5), "coefficients"), (dict(coefficients=()), "coefficients")):
         with pytest.raises(ValueError, match=message):
             muon._ns_params(kw.get("steps", 5), kw.get("coefficients", muon.COEFFICIENTS), 1e-7)
 
