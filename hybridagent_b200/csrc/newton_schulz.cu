@@ -40,7 +40,7 @@
 //
 // Measured, from call to result: 4096 x 4096 1.26 ms and 4096 x 12288 2.32 ms, 1.1 PFLOP/s executed (symmetric tiles
 // once), where the chip's power holds large fp16 products at 1.26 to 1.31; two of 17408 x 5120 10.3 ms; 128 of
-// 704 x 2816 3.9 ms, bound by the traffic of X's planes, 0.51 GB each, and by 704 in tiles of 256; 48 of 256 x 512
+// 704 x 2816 3.6 ms, bound by the traffic of X's planes, 0.51 GB each, and by 704 in tiles of 256; 48 of 256 x 512
 // 115 us and 8 of 1024 x 256 100 us, bound by the way from one stage to the next (load, products, epilogue, store,
 // counter: 4 to 8 us).
 #include <cuda.h>
@@ -331,8 +331,10 @@ __device__ __forceinline__ void store_blocks(const Args& p, Shared& sh, uint32_t
       ++tile;
       const TileAt at = tile_at(g, t);
       const int blocks = blocks_of<CG>(g, at, rank), row = at.i * (128 * CG) + rank * kBM;
+      const bool more = t + walk.step < tiles;
+      const int k0 = int((n ^ group) & 1);
       uint32_t last = kBlocks;  // block of the store before, not yet handed back
-      for (int k = int((n ^ group) & 1); k < blocks; k += 2) {
+      for (int k = k0; k < blocks; k += 2) {
         const uint32_t b = (n + k) % kBlocks, block = ring + b * kBlock, second = block + kBlocks * kBlock;
         const int col = at.j * (128 * CG) + k * kBlockCols;
         if (!mbar_wait(smem_u32(&sh.blk_ready[b]), ((n + k) / kBlocks) & 1, &sh.stop)) return;
@@ -344,20 +346,26 @@ __device__ __forceinline__ void store_blocks(const Args& p, Shared& sh, uint32_t
           if (g.epilogue <= kPoly && at.i != at.j) tma_store_3d(&p.map[g.map_2], second, row, col, at.z);
         }
         tma_store_commit();
-        if (last < kBlocks) {
-          tma_store_wait_read<1>();
-          mbar_arrive(smem_u32(&sh.blk_free[last]));
+        // With more tiles to come a block is handed back as soon as it has been read: four of them are few
+        // (3.6 ms against 4.0 for 128 of 704 x 2816).  In the last tile the next store goes first (100 us
+        // against 103 for 8 of 1024 x 256).
+        if (more) {
+          tma_store_wait_read<0>();
+          mbar_arrive(smem_u32(&sh.blk_free[b]));
+        } else {
+          if (last < kBlocks) {
+            tma_store_wait_read<1>();
+            mbar_arrive(smem_u32(&sh.blk_free[last]));
+          }
+          last = b;
         }
-        last = b;
       }
       n += blocks;
       tma_store_wait_all();
       // A tile without blocks of this group must not be counted before its matrix's previous stage is stored:
       // the counter tells stages apart only as long as they are raised one after another.
-      if (last < kBlocks)
-        mbar_arrive(smem_u32(&sh.blk_free[last]));
-      else if (!granted_wait(&sh.granted, tile, &sh.stop))
-        return;
+      if (last < kBlocks) mbar_arrive(smem_u32(&sh.blk_free[last]));
+      if (k0 >= blocks && !granted_wait(&sh.granted, tile, &sh.stop)) return;
       counter_raise(p.counter + g.counter + at.z);
     }
     walk.pass(tiles);
