@@ -68,7 +68,7 @@ constexpr int kBlocks = 4;                    // in the ring, each with room for
 constexpr int kGemmSmem = kSlots * kSlot + kBlocks * 2 * kBlock + 1024;  // + alignment
 
 // What becomes of the accumulators (times `scale`):
-//   kSymmetric  stored, with the mirrored tile (D is symmetric; tiles on and below the diagonal run)
+//   kSymmetric  stored, with the mirrored tile (D is symmetric; tiles on and above the diagonal run)
 //   kPoly       the same after adding add * addend and `diag` on the diagonal
 //   kPrecise    added to add * low, stored as high and low plane
 //   kPlain      stored
@@ -131,7 +131,8 @@ __device__ __forceinline__ float2 unpack_half2(uint32_t w) {
 struct TileAt {
   int z, i, j;  // matrix, tile row, tile column
 };
-// Tile `t` of a job.  Symmetric stages: the tiles on and below the diagonal, row by row.
+// Tile `t` of a job.  Symmetric stages: the tiles on and above the diagonal, column by column (above and not
+// below: the last column's products are only as wide as it is, the last row's always 128 or 256 rows).
 __device__ __forceinline__ TileAt tile_at(const Stage& g, int t) {
   TileAt a;
   a.z = t / g.per_matrix;
@@ -140,8 +141,8 @@ __device__ __forceinline__ TileAt tile_at(const Stage& g, int t) {
     int i = int((sqrtf(8.0f * float(r) + 1.0f) - 1.0f) * 0.5f);
     while (i * (i + 1) / 2 > r) --i;
     while ((i + 1) * (i + 2) / 2 <= r) ++i;
-    a.i = i;
-    a.j = r - i * (i + 1) / 2;
+    a.j = i;
+    a.i = r - i * (i + 1) / 2;
   } else if (g.m_fast) {
     a.j = r / g.tiles_m;
     a.i = r - a.j * g.tiles_m;
@@ -159,12 +160,17 @@ struct Walk {
   __device__ __forceinline__ void pass(int tiles) { skew = (skew + tiles) % step; }
 };
 
+// Columns of a tile that reach into D, in whole blocks: N of its products.
+template <int CG>
+__device__ __forceinline__ int width_of(const Stage& g, const TileAt& at) {
+  const int cols = g.N - at.j * (128 * CG);
+  return cols >= 128 * CG ? 128 * CG : (cols + kBlockCols - 1) & ~(kBlockCols - 1);
+}
 // Blocks of a CTA's part of a tile: those that reach into D.
 template <int CG>
 __device__ __forceinline__ int blocks_of(const Stage& g, const TileAt& at, int rank) {
   if (at.i * (128 * CG) + rank * kBM >= g.M) return 0;
-  const int cols = g.N - at.j * (128 * CG);
-  return cols >= 128 * CG ? 128 * CG / kBlockCols : (cols + kBlockCols - 1) / kBlockCols;
+  return width_of<CG>(g, at) / kBlockCols;
 }
 
 struct Shared {
@@ -372,8 +378,8 @@ __device__ __forceinline__ void store_blocks(const Args& p, Shared& sh, uint32_t
   }
 }
 
-// CG: CTAs of a tile (1: 128 x 128; 2: 256 x 256, each CTA with 128 rows of A and of D and 128 columns
-// of B).
+// CG: CTAs of a tile (1: 128 x 128; 2: 256 x 256, each CTA with 128 rows of A and of D and half of the
+// columns of B).
 template <int CG, class Args>
 __global__ void __launch_bounds__(kGemmThreads, 1) newton_schulz_kernel(const __grid_constant__ Args p) {
   constexpr int kTile = 128 * CG;         // rows and columns of a tile
@@ -434,7 +440,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1) newton_schulz_kernel(const __
             ready = at.z;
           }
           grant(&sh.granted, ++tile);
-          const int m0 = at.i * kTile + int(rank) * kBM, n0 = at.j * kTile + int(rank) * 128;
+          const int m0 = at.i * kTile + int(rank) * kBM;
+          const int n0 = at.j * kTile + (CG == 2 ? int(rank) * (width_of<CG>(g, at) / 2) : 0);
           for (int kb = 0; kb < kblocks; ++kb) {
             ok = mbar_wait(smem_u32(&sh.empty[slot]), phase ^ 1, &sh.stop);
             if (!ok) break;
@@ -471,10 +478,11 @@ __global__ void __launch_bounds__(kGemmThreads, 1) newton_schulz_kernel(const __
         const Stage& g = p.stage[job.stage];
         const int tiles = job.count * g.per_matrix;
         const int kblocks = (g.K + kBK - 1) / kBK;
-        const uint32_t idesc = f16_idesc(kTile, kTile, g.a_mn, g.b_mn);
         const uint32_t lead_a = g.a_mn ? 8192 : 16, lead_b = g.b_mn ? 8192 : 16;
         const uint32_t next_a = g.a_mn ? kStepMN : kStepK, next_b = g.b_mn ? kStepMN : kStepK;
         for (int t = walk.start(); t < tiles && ok; t += walk.step) {
+          const int width = g.N % kTile == 0 ? kTile : width_of<CG>(g, tile_at(g, t));
+          const uint32_t idesc = f16_idesc(kTile, width, g.a_mn, g.b_mn);
           ok = mbar_wait(smem_u32(&sh.acc_empty[acc]), acc_phase ^ 1, &sh.stop);
           if (!ok) break;
           tc_fence_after();
@@ -738,7 +746,8 @@ bool cut(Stage* stages, int count, int64_t batch, int cg, int workers, double* w
     before += uint32_t(per) * 2 * cg;   // both store warps of each of its CTAs
     const double tiles = double(per * batch), each = (cg == 1 ? 500.0 : 600.0) * ((g.K + kBK - 1) / kBK);
     const double wait = cg == 1 ? 8e3 : 16e3;
-    *work += each * tiles / workers;
+    const double spared = double(g.tiles_n * tile - g.N) / tile * double(g.tiles_m * batch);  // in the last column
+    *work += each * (tiles - spared) / workers;
     *alone += each * double((per * batch + workers - 1) / workers) + (tiles > workers ? wait * workers / tiles : wait);
   }
   return true;
