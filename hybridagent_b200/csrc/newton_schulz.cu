@@ -13,8 +13,14 @@
 // in five steps).  So the first kPreciseSteps steps keep X as a high and a low fp16 plane (22 bits).
 // The products read the high plane only: with a on B's diagonal a step is (a I + B) X, and its
 // epilogue adds a * low in fp32 (what B does to the low plane touches only the few leading
-// directions).  Against 64-bit results (rank-16 plus 5 % noise, 1024 x 1024, rounded to bf16): 2.2e-3
+// directions).  Against 64-bit results (rank-16 plus 5 % noise, 1024 x 1024, rounded to bf16): 2.1e-3
 // relative, of which 1.7e-3 is the final rounding; one fp16 plane gives 2.1e-2, bf16 operands 1.6e-1.
+//
+// The diagonals of G and of the factors keep what their rounding takes, in fp32 (diagonal_at below).  Where all
+// singular values are alike, as in a matrix much longer than wide, these matrices are close to multiples of I, their
+// diagonals round in the same direction, and the later steps amplify that up to fourfold: 383 x 14575, normal
+// elements, is 2.95e-3 off without and 1.78e-3 with it (rounded to bf16).  It costs 3 us of the 116 of 48 of
+// 256 x 512 and under 1 % of large batches.
 //
 // Two steps can run as one product with X: with Q1 = a I + b G + c G^2 (G = X X^T), the Gram matrix
 // after the step is G' = Q1 G Q1 (all three commute), Q2 follows from G', and X <- (Q2 Q1) X.  That
@@ -40,8 +46,8 @@
 //
 // Measured, from call to result: 4096 x 4096 1.26 ms and 4096 x 12288 2.32 ms, 1.1 PFLOP/s executed (symmetric tiles
 // once), where the chip's power holds large fp16 products at 1.26 to 1.31; two of 17408 x 5120 10.3 ms; 128 of
-// 704 x 2816 3.6 ms, bound by the traffic of X's planes, 0.51 GB each, and by 704 in tiles of 256; 48 of 256 x 512
-// 115 us and 8 of 1024 x 256 100 us, bound by the way from one stage to the next (load, products, epilogue, store,
+// 704 x 2816 3.5 ms, bound by the traffic of X's planes, 0.51 GB each, and by 704 in tiles of 256; 48 of 256 x 512
+// 120 us and 8 of 1024 x 256 103 us, bound by the way from one stage to the next (load, products, epilogue, store,
 // counter: 4 to 8 us).
 #include <cuda.h>
 
@@ -95,7 +101,10 @@ struct Stage {
   int counter;        // of the shape's first matrix
   float scale, add, diag;
   uint8_t map_a, map_b, map_out, map_2, map_add;
-  int8_t epilogue, m_fast, a_mn, b_mn, keep_low;  // *_mn: the operand's M / N index is the contiguous one
+  int8_t square_1, square_2, square_out;  // the square matrices read and written, or -1
+  float4* diagonal;     // of the shape's square matrices: square i of matrix z at i * diagonal_all + z * diagonal_each
+  int diagonal_each, diagonal_all;
+  int8_t epilogue, m_fast, a_mn, b_mn, keep_low, by_column;  // *_mn: the operand's M / N index is the contiguous one
 };
 // A stage of all `count` matrices of its shape.
 struct Job {
@@ -131,6 +140,17 @@ __device__ __forceinline__ float2 unpack_half2(uint32_t w) {
 struct TileAt {
   int z, i, j;  // matrix, tile row, tile column
 };
+// A square matrix's diagonal element q = r + e, r its fp16 value, as (r, e, e / r).  To first order and on the
+// diagonal alone, a product gains e1 r2 + r1 e2 there.  In the product with X, row (tall: column) i should gain
+// e x_i; it is scaled by 1 + e / r, which is the same for what the diagonal contributes.
+__device__ __forceinline__ float4* diagonal_at(const Stage& g, int square, int z, int row) {
+  return g.diagonal + int64_t(square) * g.diagonal_all + int64_t(z) * g.diagonal_each + row;
+}
+__device__ __forceinline__ float4 split_diagonal(float q) {
+  const float r = __half2float(__float2half_rn(q)), e = q - r;
+  const float f = __fdividef(e, r);  // at most half a step; more, or NaN, where r is subnormal or 0
+  return make_float4(r, e, fabsf(f) <= 1.0f / 2048 ? f : 0.0f, 0.0f);
+}
 // Tile `t` of a job.  Symmetric stages: the tiles on and above the diagonal, column by column (above and not
 // below: the last column's products are only as wide as it is, the last row's always 128 or 256 rows).
 __device__ __forceinline__ TileAt tile_at(const Stage& g, int t) {
@@ -188,7 +208,7 @@ struct Warp {
   Walk walk;
   uint32_t ring;           // shared memory: blocks, then their second results
   uint32_t tmem;           // its lanes of the accumulators
-  uint32_t n;              // blocks of this CTA so far
+  uint32_t n, tile;        // blocks and tiles of this CTA so far
   uint32_t acc, acc_phase;
 };
 
@@ -200,17 +220,72 @@ __device__ __forceinline__ bool epilogue(const Stage& g, const Job& job, Warp& w
   const int lane = w.lane;
   const int mine = w.quarter * 32 + lane;                            // this lane's row of a block:
   const uint32_t row_at = mine * 64, key = (uint32_t(mine) >> 1) & 3;  // its 16-byte piece j lies at j ^ key
-  const float scale = g.scale, add_scale = g.add, diag = g.diag;
+  const float add_scale = g.add;
   const int tiles = job.count * g.per_matrix;
+  // Of the diagonals: (r, e) of this lane's row from both factors; factor of its row of X, or of its columns in
+  // the group's blocks.
+  float d[kSym ? 4 : 2 * CG];
+  auto fetch = [&](const TileAt& at, int k0) {
+    if (!kSym && g.by_column) {
+#pragma unroll
+      for (int u = 0; u < 2 * CG; ++u) {
+        const int col = at.j * kTile + (k0 + 2 * u) * kBlockCols + lane;
+        d[u] = col < g.N ? __ldcg(&diagonal_at(g, g.square_1, at.z, col)->z) : 0.0f;
+      }
+    } else {
+      const int row = at.i * kTile + w.rank * kBM + mine;
+      if (kSym) {
+        float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f), b = a;
+        if (row < g.M) {
+          a = __ldcg(diagonal_at(g, g.square_1, at.z, row));
+          b = __ldcg(diagonal_at(g, g.square_2, at.z, row));
+        }
+        d[0] = a.x, d[1] = a.y, d[2 * kSym] = b.x, d[3 * kSym] = b.y;
+      } else {
+        d[0] = row < g.M ? __ldcg(&diagonal_at(g, g.square_1, at.z, row)->z) : 0.0f;
+      }
+    }
+  };
+  auto wanted = [&](const TileAt& at) { return g.square_1 >= 0 && (!kSym || at.i == at.j); };
+  bool fetched = false;
   for (int t = w.walk.start(); t < tiles; t += w.walk.step) {
     const TileAt at = tile_at(g, t);
     const int blocks = blocks_of<CG>(g, at, w.rank);
-    const int row = at.i * kTile + w.rank * kBM + mine;
+    const int row = at.i * kTile + w.rank * kBM + mine, k0 = int((w.n ^ uint32_t(w.group)) & 1);
+    float scale = g.scale, diag = g.diag;
+    __half2 by_column[CG];  // factors less 1
+    ++w.tile;
+    if (wanted(at)) {
+      if (!fetched) {
+        bool ok = true;
+        if (lane == 0) ok = granted_wait(&sh.granted, w.tile, &sh.stop);
+        if (!__all_sync(0xffffffffu, ok)) return false;
+        fetch(at, k0);
+      }
+      if (kSym) {
+        diag += EPI == kPoly ? d[1] * (add_scale + 2.0f * scale * d[0])
+                             : scale * (d[0] * d[3 * kSym] + d[1] * d[2 * kSym]);
+      } else if (!g.by_column) {
+        scale *= 1.0f + d[0];
+      } else {
+#pragma unroll
+        for (int u = 0; u < CG; ++u) by_column[u] = __floats2half2_rn(d[2 * u], d[2 * u + 1]);
+      }
+    }
+    // The next tile's, if it may be read already: loaded while this one is worked on.
+    fetched = false;
+    if (t + w.walk.step < tiles) {
+      const TileAt next = tile_at(g, t + w.walk.step);
+      if (wanted(next) && __all_sync(0xffffffffu, lane != 0 || granted_now(&sh.granted) > w.tile)) {
+        fetch(next, k0 ^ (blocks & 1));
+        fetched = true;
+      }
+    }
     if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&sh.acc_full[w.acc]), w.acc_phase, &sh.stop))) return false;
     tc_fence_after();
     const uint32_t d = w.tmem + w.acc * kTile;
 #pragma unroll 1
-    for (int k = int((w.n ^ uint32_t(w.group)) & 1); k < blocks; k += 2) {
+    for (int k = k0; k < blocks; k += 2) {
       const uint32_t b = (w.n + k) % kBlocks, phase = ((w.n + k) / kBlocks) & 1;
       const uint32_t block = w.ring + b * kBlock, second = block + kBlocks * kBlock;
       const int col = at.j * kTile + k * kBlockCols;
@@ -227,7 +302,12 @@ __device__ __forceinline__ bool epilogue(const Stage& g, const Job& job, Warp& w
                        : "memory");
       }
       tmem_ld_wait();
-      uint32_t out[16], low[16];  // 32 packed results
+      if (!kSym && g.by_column) {
+        const __half2 two = CG == 2 && k >= 4 ? by_column[CG - 1] : by_column[0];
+        const float f = 1.0f + ((k & 2) ? __high2float(two) : __low2float(two));
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) * __shfl_sync(0xffffffffu, f, j));
+      }
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
         float x = __uint_as_float(v[2 * j]) * scale, y = __uint_as_float(v[2 * j + 1]) * scale;
@@ -236,10 +316,26 @@ __device__ __forceinline__ bool epilogue(const Stage& g, const Job& job, Warp& w
           x = __fmaf_rn(add_scale, a.x, x);
           y = __fmaf_rn(add_scale, a.y, y);
         }
-        if (EPI == kPoly) {
-          if (col + 2 * j == row) x += diag;
-          if (col + 2 * j + 1 == row) y += diag;
-        }
+        v[2 * j] = __float_as_uint(x);
+        v[2 * j + 1] = __float_as_uint(y);
+      }
+      if (kSym && col == row - lane && at.i == at.j) {  // lane l's element l is on the diagonal
+        float mine = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+          if (j == lane) {
+            mine = __uint_as_float(v[j]) + diag;
+            v[j] = __float_as_uint(mine);
+          }
+        const float4 q = split_diagonal(mine);  // where a tile off the diagonal has its mirrored block
+        asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(second + lane * 16), "f"(q.x), "f"(q.y),
+                     "f"(q.z), "f"(q.w)
+                     : "memory");
+      }
+      uint32_t out[16], low[16];  // 32 packed results
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const float x = __uint_as_float(v[2 * j]), y = __uint_as_float(v[2 * j + 1]);
         if (EPI == kFinal) {
           const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
           out[j] = *reinterpret_cast<const uint32_t*>(&h);
@@ -349,7 +445,11 @@ __device__ __forceinline__ void store_blocks(const Args& p, Shared& sh, uint32_t
           if (g.keep_low) tma_store_3d(&p.map[g.map_2], block, col, row, at.z);
         } else {
           tma_store_3d(&p.map[g.map_out], block, col, row, at.z);
-          if (g.epilogue <= kPoly && at.i != at.j) tma_store_3d(&p.map[g.map_2], second, row, col, at.z);
+          if (g.epilogue <= kPoly && at.i != at.j) {
+            tma_store_3d(&p.map[g.map_2], second, row, col, at.z);
+          } else if (g.epilogue <= kPoly && col >= row && col < row + kBM) {  // the block holds 32 diagonal elements
+            bulk_store(diagonal_at(g, g.square_out, at.z, col), second, kBlockCols * sizeof(float4));
+          }
         }
         tma_store_commit();
         // With more tiles to come a block is handed back as soon as it has been read: four of them are few
@@ -604,9 +704,9 @@ int sm_count(int* out) {
 
 // How many of the leading pairs of steps, (0, 1) and (2, 3), run as one product with X.  Each saves
 // 3 m^2 (n - m) multiply-adds and costs a stage.  Relative error against 64-bit results (CPU model
-// of these roundings, rounded to bf16; none / first / both): 1024 x 4096 normal 1.85 / 1.86 / 2.15e-3,
-// 512 x 1536 2.16 / 2.18 / 2.57e-3, rank 16 plus 5 % noise 1024 x 4096 2.18 / 2.21 / 2.36e-3: the first
-// pair costs nothing, the second little where m is large.
+// of these roundings, rounded to bf16; first / both): 700 x 2816 normal 1.81 / 2.16e-3, 1100 x 2200 1.80 / 2.14e-3,
+// rank 16 plus 5 % noise 700 x 2816 1.76 / 1.83e-3; none / first: 256 x 512 1.94 / 1.94e-3: the first pair costs
+// nothing, the second little where m is large.
 int pairs(int64_t m, int64_t n, const float* coef, int steps) {
   int count = 0;
   double top = 1.0;  // bound of the singular values before step s
@@ -658,6 +758,10 @@ int make_stages(NsBatch* shape, const float* coef, int steps, int map0, int coun
     g.counter = counter;
     g.epilogue = int8_t(e);
     g.M = M, g.N = N, g.K = K;
+    g.square_1 = g.square_2 = g.square_out = -1;
+    g.diagonal = b.diagonal[0];
+    g.diagonal_each = int(b.m_pad);
+    g.diagonal_all = int(b.m_pad * b.n);
     return &g;
   };
   // a symmetric m x m product of square matrices x and y, which commute
@@ -668,6 +772,9 @@ int make_stages(NsBatch* shape, const float* coef, int steps, int map0, int coun
     g->map_out = uint8_t(map0 + kMapSqOut + to);
     g->map_2 = uint8_t(map0 + kMapSqMirror + to);
     g->map_add = uint8_t(map0 + kMapSqOut + x);
+    g->square_1 = int8_t(x);
+    g->square_2 = int8_t(y);
+    g->square_out = int8_t(to);
     g->scale = 1.0f / kScaleG;
     return g;
   };
@@ -687,6 +794,7 @@ int make_stages(NsBatch* shape, const float* coef, int steps, int map0, int coun
     g->map_a = g->map_b = uint8_t(map0 + (tall ? kMapXmn : kMapXk) + cur);
     g->map_out = uint8_t(map0 + kMapSqOut);
     g->map_2 = uint8_t(map0 + kMapSqMirror);
+    g->square_out = 0;
     g->scale = kScaleG / (kScaleX * kScaleX);
     factor(0, 1, c);
     if (pair) {
@@ -698,6 +806,8 @@ int make_stages(NsBatch* shape, const float* coef, int steps, int map0, int coun
     const int q = pair ? 0 : 1;
     g = add(s < kPreciseSteps ? kPrecise : kPlain, int(b.rows), int(b.cols), m);
     g->b_mn = !tall;
+    g->by_column = tall;
+    g->square_1 = int8_t(q);
     g->map_a = uint8_t(map0 + (tall ? kMapXk + cur : kMapSq + q));
     g->map_b = uint8_t(map0 + (tall ? kMapSq + q : kMapXmn + cur));
     cur ^= 1;
@@ -873,7 +983,7 @@ double ns_factor(const float* c, double s) {
 
 int64_t ns_bytes_per_matrix(int64_t rows, int64_t cols) {
   const int64_t m = rows < cols ? rows : cols;
-  return up(rows * up(cols, 8) * 2, 256) * 3 + up(m * up(m, 8) * 2, 256) * 3;
+  return up(rows * up(cols, 8) * 2, 256) * 3 + (up(m * up(m, 8) * 2, 256) + up(m, 32) * int64_t(sizeof(float4))) * 3;
 }
 
 void ns_carve(NsBatch* b, void* base) {
@@ -887,6 +997,9 @@ void ns_carve(NsBatch* b, void* base) {
   b->hi[1] = b->hi[0] + b->n * b->plane_x;
   b->lo = b->hi[1] + b->n * b->plane_x;
   for (int i = 0; i < 3; ++i) b->square[i] = b->lo + b->n * b->plane_x + i * b->n * b->plane_g;
+  b->m_pad = up(b->m, 32);
+  float4* d = reinterpret_cast<float4*>(b->square[2] + b->n * b->plane_g);
+  for (int i = 0; i < 3; ++i) b->diagonal[i] = d + i * b->n * b->m_pad;
 }
 
 int ns_stages(int steps) { return 3 * steps + 2; }

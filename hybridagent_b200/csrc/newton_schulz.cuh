@@ -24,6 +24,8 @@ struct NsBatch {
   int64_t plane_x, plane_g;      // elements of one matrix
   __half *hi[2], *lo;            // X before and after a step; low plane
   __half* square[3];             // m x m: Gram matrices and factors
+  float4* diagonal[3];           // what rounding took from their diagonals, m_pad elements for each matrix
+  int64_t m_pad;
   uint32_t* counter;             // one for each matrix, zero before the run
   uint32_t* error;               // set to 1 if a wait ran out
   bool bf16;                     // the result is wanted as bf16 (a run of this shape alone) ...

@@ -125,12 +125,15 @@ __device__ __forceinline__ bool counter_wait(const uint32_t* counter, uint32_t w
 __device__ __forceinline__ void grant(uint32_t* granted, uint32_t value) {
   asm volatile("st.release.cta.shared::cta.u32 [%0], %1;" ::"r"(smem_u32(granted)), "r"(value) : "memory");
 }
+__device__ __forceinline__ uint32_t granted_now(uint32_t* granted) {
+  uint32_t v;
+  asm volatile("ld.acquire.cta.shared::cta.u32 %0, [%1];" : "=r"(v) : "r"(smem_u32(granted)) : "memory");
+  return v;
+}
 __device__ __forceinline__ bool granted_wait(uint32_t* granted, uint32_t want, volatile uint32_t* stop) {
   const uint64_t t0 = global_ns();
   for (uint32_t i = 1;; ++i) {
-    uint32_t v;
-    asm volatile("ld.acquire.cta.shared::cta.u32 %0, [%1];" : "=r"(v) : "r"(smem_u32(granted)) : "memory");
-    if (v >= want) break;
+    if (granted_now(granted) >= want) break;
     if ((i & 255) == 0) {
       if (*stop) return false;
       if (global_ns() - t0 > kWaitNs) {
@@ -172,6 +175,13 @@ __device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, uint32_t sr
   asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(
                    reinterpret_cast<uint64_t>(map)),
                "r"(src), "r"(x), "r"(y), "r"(z)
+               : "memory");
+}
+// Plain bytes; addresses and size are multiples of 16.
+__device__ __forceinline__ void bulk_store(void* dst, uint32_t src, uint32_t bytes) {
+  asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(
+                   static_cast<uint64_t>(__cvta_generic_to_global(dst))),
+               "r"(src), "r"(bytes)
                : "memory");
 }
 __device__ __forceinline__ void tma_store_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }

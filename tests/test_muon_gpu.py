@@ -576,3 +576,23 @@ def test_a_step_that_gave_up_is_reported():
     set_grads(params, 1, torch.bfloat16)
     with pytest.raises(RuntimeError, match="ran out"):
         opt.step()
+
+
+@pytest.mark.parametrize("shape", [(1, 383, 14575), (2, 11249, 366), (3, 2000, 140), (1, 742, 1520), (2, 260, 260)])
+def test_matrices_whose_singular_values_are_alike(shape):
+    """They round the diagonals of all Gram matrices and factors the same way, unless those are kept.  What the fp16
+    planes leave then, 2^-11 in elements of random sign, is less than the bf16 result's own rounding, 2^-8."""
+    import torch
+    from hybridagent_b200 import orthogonalize
+    x = values("normal", shape, torch.float32, seed=sum(shape))
+    want = definition(x)
+    assert off(orthogonalize(x), want) <= 1.5 * off(want.bfloat16(), want)
+
+
+def test_orthogonal_matrices_stay_so():
+    import torch
+    from hybridagent_b200 import orthogonalize
+    for rows, cols in ((300, 300), (200, 1100), (1500, 700), (129, 5000)):
+        x = torch.linalg.qr(values("normal", (max(rows, cols), min(rows, cols)), torch.float32, seed=rows))[0]
+        x = (x if rows >= cols else x.mT).contiguous()
+        assert off(orthogonalize(x), definition(x)) <= NS_BF16
