@@ -706,12 +706,12 @@ int sm_count(int* out) {
 // 3 m^2 (n - m) multiply-adds and costs a stage.  Relative error against 64-bit results (CPU model
 // of these roundings, rounded to bf16; first / both): 700 x 2816 normal 1.81 / 2.16e-3, 1100 x 2200 1.80 / 2.14e-3,
 // rank 16 plus 5 % noise 700 x 2816 1.76 / 1.83e-3; none / first: 256 x 512 1.94 / 1.94e-3: the first pair costs
-// nothing, the second little where m is large.
+// nothing, the second little where m is large.  On the GPU, the worst of 35 normal 640 x 1280: 2.51e-3 with both.
 int pairs(int64_t m, int64_t n, const float* coef, int steps) {
   int count = 0;
   double top = 1.0;  // bound of the singular values before step s
   for (int s = 0; s + 2 <= steps && s < 4; s += 2) {
-    const bool worth = s == 0 ? n * 2 >= m * 3 && m >= 256 : n >= m * 2 && m >= 640;
+    const bool worth = s == 0 ? n * 2 >= m * 3 && m >= 256 : n >= m * 2 && m >= (n >= m * 3 ? 640 : 768);
     const double between = ns_growth(coef + 3 * s, top);
     // both factors' product has to fit the planes like each of them
     if (!worth || ns_factor(coef + 3 * s, top) * ns_factor(coef + 3 * s + 3, between) > kMaxFactor) break;

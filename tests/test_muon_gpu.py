@@ -578,7 +578,8 @@ def test_a_step_that_gave_up_is_reported():
         opt.step()
 
 
-@pytest.mark.parametrize("shape", [(1, 383, 14575), (2, 11249, 366), (3, 2000, 140), (1, 742, 1520), (2, 260, 260)])
+@pytest.mark.parametrize("shape", [(1, 383, 14575), (2, 11249, 366), (3, 2000, 140), (1, 742, 1520), (2, 260, 260),
+                                   (35, 640, 1280), (20, 769, 1700), (24, 1600, 704), (30, 544, 352)])
 def test_matrices_whose_singular_values_are_alike(shape):
     """They round the diagonals of all Gram matrices and factors the same way, unless those are kept.  What the fp16
     planes leave then, 2^-11 in elements of random sign, is less than the bf16 result's own rounding, 2^-8."""
