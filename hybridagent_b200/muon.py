@@ -24,6 +24,7 @@ exact iteration, of which rounding to bf16 is 1.7e-3.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 import operator
 import os
@@ -55,6 +56,12 @@ def _ns_params(steps: int, coefficients, eps: float) -> _lib.NsParams:
     return out
 
 
+@functools.lru_cache(maxsize=64)
+def _usual_params(steps: int, eps: float) -> _lib.NsParams:
+    return _ns_params(steps, COEFFICIENTS, eps)
+
+
+@functools.lru_cache(maxsize=4096)
 def _workspace_bytes(batch: int, rows: int, cols: int) -> int:
     out = ctypes.c_size_t(0)
     _lib.call("ha_orthogonalize_workspace", batch, rows, cols, ctypes.byref(out))
@@ -68,7 +75,6 @@ def _budget(name: str, default: int) -> int:
     return value
 
 
-@torch.no_grad()
 def orthogonalize(x: torch.Tensor, *, steps: int = 5, coefficients=COEFFICIENTS, eps: float = 1e-7,
                   out: torch.Tensor | None = None) -> torch.Tensor:
     """The Newton-Schulz orthogonalisation of ``x`` (..., rows, cols), each matrix for itself, as bf16.
@@ -88,7 +94,12 @@ def orthogonalize(x: torch.Tensor, *, steps: int = 5, coefficients=COEFFICIENTS,
     if x.device.type != "cuda":
         raise RuntimeError(f"orthogonalize runs on CUDA devices only; the tensor is on {x.device} "
                            "(there is no CPU path)")
-    ns = _ns_params(steps, coefficients, eps)
+    if coefficients is COEFFICIENTS and type(steps) is int and type(eps) is float:
+        ns = _usual_params(steps, eps)
+    else:
+        ns = _ns_params(steps, coefficients, eps)
+    if x.requires_grad:
+        x = x.detach()
     if out is not None:
         if out.dtype != torch.bfloat16 or out.shape != x.shape or out.device != x.device or not out.is_contiguous():
             raise ValueError(f"out must be a contiguous bfloat16 tensor of shape {tuple(x.shape)} on {x.device}")
@@ -103,12 +114,19 @@ def orthogonalize(x: torch.Tensor, *, steps: int = 5, coefficients=COEFFICIENTS,
     if src.numel() == 0:
         return out
     batch = src.numel() // (rows * cols)
-    need, one = _workspace_bytes(batch, rows, cols), _workspace_bytes(1, rows, cols)
-    size = min(need, max(one, _budget("HYBRIDAGENT_B200_NS_BYTES", 8 << 30)))
-    with torch.cuda.device(x.device):
-        ws = torch.empty(size, dtype=torch.uint8, device=x.device)
-        _lib.call("ha_orthogonalize", src.data_ptr(), _CODES[x.dtype], out.data_ptr(), batch, rows, cols,
-                  ctypes.byref(ns), ws.data_ptr(), size, torch.cuda.current_stream().cuda_stream)
+    size = _workspace_bytes(batch, rows, cols)
+    budget = _budget("HYBRIDAGENT_B200_NS_BYTES", 8 << 30)
+    if size > budget:
+        size = min(size, max(budget, _workspace_bytes(1, rows, cols)))
+    ws = torch.empty(size, dtype=torch.uint8, device=x.device)
+    device = x.device.index
+    args = ("ha_orthogonalize", src.data_ptr(), _CODES[x.dtype], out.data_ptr(), batch, rows, cols, ctypes.byref(ns),
+            ws.data_ptr(), size, torch._C._cuda_getCurrentRawStream(device))
+    if device == torch._C._cuda_getDevice():
+        _lib.call(*args)
+    else:
+        with torch.cuda.device(device):
+            _lib.call(*args)
     return out
 
 
