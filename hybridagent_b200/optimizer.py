@@ -91,6 +91,20 @@ _TORCH = {v: k for k, v in _CODES.items()}
 STATE_FORMAT = "hybridagent_b200.zero1_adamw/1"
 
 
+_STREAMS: dict[tuple[int, int], torch.cuda.Stream] = {}
+
+
+def _current_stream() -> torch.cuda.Stream:
+    """The current device's current stream.  Its object is kept by device and handle: torch makes a new one at every
+    call, which takes the host several microseconds."""
+    device = torch._C._cuda_getDevice()
+    key = (device, torch._C._cuda_getCurrentRawStream(device))
+    stream = _STREAMS.get(key)
+    if stream is None:
+        stream = _STREAMS[key] = torch.cuda.current_stream()
+    return stream
+
+
 class _Table:
     """A host table (numpy structured array) mirrored in device memory.
 
@@ -120,7 +134,7 @@ class _Table:
             ev.synchronize()
         np.copyto(self._views[k], self._bytes)
         self.dev.copy_(self._ring[k], non_blocking=True)
-        ev.record()
+        ev.record(_current_stream())
 
     @property
     def ptr(self) -> int:
@@ -1175,7 +1189,7 @@ class ZeroOneAdamW:
         tables while the copy is in flight (if they are not yet), and returns the sums."""
         host.copy_(dev, non_blocking=True)
         ev = torch.cuda.Event()
-        ev.record()
+        ev.record(_current_stream())
         if stage:
             self._stage_step()
         ev.synchronize()
@@ -1257,7 +1271,7 @@ class ZeroOneAdamW:
             self.dense_steps += dense
             self._phase("adamw", True)
             ce_gather = p2p and self.gather_mode == "ce"
-            main = torch.cuda.current_stream()
+            main = _current_stream()
             for c, sc in sorted(launches, key=lambda item: not item[0].muon):  # the longest work first
                 chunks, n = c.adamw_chunks
                 if c.changed_event is not None and c.changed_event.query():  # the last count has landed
@@ -1301,7 +1315,7 @@ class ZeroOneAdamW:
                 if changed_only:
                     c.changed_host.copy_(c.changed_dev, non_blocking=True)
                     c.changed_event = torch.cuda.Event()
-                    c.changed_event.record()
+                    c.changed_event.record(main)
             for st in self._gather_streams:
                 main.wait_stream(st)
             self._phase("adamw", False)
