@@ -23,9 +23,12 @@
 // 256 x 512 and under 1 % of large batches.
 //
 // Two steps can run as one product with X: with Q1 = a I + b G + c G^2 (G = X X^T), the Gram matrix
-// after the step is G' = Q1 G Q1 (all three commute), Q2 follows from G', and X <- (Q2 Q1) X.  That
-// replaces two products with X (6 m^2 n of 2 (3 m^2 n + m^3)) by one and three more symmetric ones:
-// 3 m^2 n + 5 m^3.  See pairs() for where that is done and what it costs in accuracy.
+// after the step is G' = Q1 G Q1, Q2 follows from G', and X <- (Q2 Q1) X.  That replaces 2 (3 m^2 n + m^3)
+// operations by 3 m^2 n + 7 m^3.  All of these are polynomials of G and commute, but once rounded they do not: Q1 G
+// and Q2 Q1 are not symmetric and are formed in full.  Mirroring one half of them puts their commutators, as large as the
+// roundings, into directions that X has not, where the steps multiply them: 2.3e-2 instead of 5.2e-3 for a matrix
+// 4096 x 12288 of rank 32.  Q1 (Q1 G)^T is symmetric up to the rounding of Q1 G.  See pairs() for where steps
+// are merged and what that costs in accuracy.
 //
 // All products of all steps of all shapes run in one persistent launch, one CTA per SM, one or two CTAs to a
 // tile: a step of a small matrix takes a few microseconds, less than what three launches cost.  The work is a list of
@@ -74,12 +77,13 @@ constexpr int kBlocks = 4;                    // in the ring, each with room for
 constexpr int kGemmSmem = kSlots * kSlot + kBlocks * 2 * kBlock + 1024;  // + alignment
 
 // What becomes of the accumulators (times `scale`):
-//   kSymmetric  stored, with the mirrored tile (D is symmetric; tiles on and above the diagonal run)
+//   kSquare     stored, of square matrices; with the mirrored tile where the stage says so (tiles on and above
+//               the diagonal run)
 //   kPoly       the same after adding add * addend and `diag` on the diagonal
 //   kPrecise    added to add * low, stored as high and low plane
 //   kPlain      stored
 //   kFinal      stored as bf16
-enum Epilogue { kSymmetric, kPoly, kPrecise, kPlain, kFinal };
+enum Epilogue { kSquare, kPoly, kPrecise, kPlain, kFinal };
 
 // Tensor maps of a run: per buffer, the boxes it is read and written in.
 enum Map {
@@ -105,6 +109,7 @@ struct Stage {
   float4* diagonal;     // of the shape's square matrices: square i of matrix z at i * diagonal_all + z * diagonal_each
   int diagonal_each, diagonal_all;
   int8_t epilogue, m_fast, a_mn, b_mn, keep_low, by_column;  // *_mn: the operand's M / N index is the contiguous one
+  int8_t mirror;        // D is symmetric
 };
 // A stage of all `count` matrices of its shape.
 struct Job {
@@ -151,13 +156,13 @@ __device__ __forceinline__ float4 split_diagonal(float q) {
   const float f = __fdividef(e, r);  // at most half a step; more, or NaN, where r is subnormal or 0
   return make_float4(r, e, fabsf(f) <= 1.0f / 2048 ? f : 0.0f, 0.0f);
 }
-// Tile `t` of a job.  Symmetric stages: the tiles on and above the diagonal, column by column (above and not
+// Tile `t` of a job.  Mirrored stages: the tiles on and above the diagonal, column by column (above and not
 // below: the last column's products are only as wide as it is, the last row's always 128 or 256 rows).
 __device__ __forceinline__ TileAt tile_at(const Stage& g, int t) {
   TileAt a;
   a.z = t / g.per_matrix;
   const int r = t - a.z * g.per_matrix;
-  if (g.epilogue <= kPoly) {
+  if (g.mirror) {
     int i = int((sqrtf(8.0f * float(r) + 1.0f) - 1.0f) * 0.5f);
     while (i * (i + 1) / 2 > r) --i;
     while ((i + 1) * (i + 2) / 2 <= r) ++i;
@@ -214,7 +219,7 @@ struct Warp {
 
 template <int CG, int EPI>
 __device__ __forceinline__ bool epilogue(const Stage& g, const Job& job, Warp& w, Shared& sh) {
-  constexpr bool kSym = EPI == kSymmetric || EPI == kPoly;
+  constexpr bool kSym = EPI == kSquare || EPI == kPoly;
   constexpr bool kAdd = EPI == kPoly || EPI == kPrecise;
   constexpr int kTile = 128 * CG;
   const int lane = w.lane;
@@ -358,7 +363,7 @@ __device__ __forceinline__ bool epilogue(const Stage& g, const Job& job, Warp& w
                        "r"(out[4 * j]), "r"(out[4 * j + 1]), "r"(out[4 * j + 2]), "r"(out[4 * j + 3])
                        : "memory");
       }
-      if (kSym && at.i != at.j) {
+      if (kSym && g.mirror && at.i != at.j) {
         // transposed, 32 rows of 128: lanes 2l and 2l + 1 exchange halves so that each writes two
         // neighbours of one row
 #pragma unroll
@@ -445,9 +450,9 @@ __device__ __forceinline__ void store_blocks(const Args& p, Shared& sh, uint32_t
           if (g.keep_low) tma_store_3d(&p.map[g.map_2], block, col, row, at.z);
         } else {
           tma_store_3d(&p.map[g.map_out], block, col, row, at.z);
-          if (g.epilogue <= kPoly && at.i != at.j) {
-            tma_store_3d(&p.map[g.map_2], second, row, col, at.z);
-          } else if (g.epilogue <= kPoly && col >= row && col < row + kBM) {  // the block holds 32 diagonal elements
+          if (at.i != at.j) {
+            if (g.mirror) tma_store_3d(&p.map[g.map_2], second, row, col, at.z);
+          } else if (g.square_out >= 0 && col >= row && col < row + kBM) {  // the block holds 32 diagonal elements
             bulk_store(diagonal_at(g, g.square_out, at.z, col), second, kBlockCols * sizeof(float4));
           }
         }
@@ -629,7 +634,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) newton_schulz_kernel(const __
       const Job job = p.job[q];
       const Stage& g = p.stage[job.stage];
       switch (g.epilogue) {
-        case kSymmetric: ok = epilogue<CG, kSymmetric>(g, job, w, sh); break;
+        case kSquare: ok = epilogue<CG, kSquare>(g, job, w, sh); break;
         case kPoly: ok = epilogue<CG, kPoly>(g, job, w, sh); break;
         case kPrecise: ok = epilogue<CG, kPrecise>(g, job, w, sh); break;
         case kPlain: ok = epilogue<CG, kPlain>(g, job, w, sh); break;
@@ -702,16 +707,21 @@ int sm_count(int* out) {
   return HA_OK;
 }
 
-// How many of the leading pairs of steps, (0, 1) and (2, 3), run as one product with X.  Each saves
-// 3 m^2 (n - m) multiply-adds and costs a stage.  Relative error against 64-bit results (CPU model
-// of these roundings, rounded to bf16; first / both): 700 x 2816 normal 1.81 / 2.16e-3, 1100 x 2200 1.80 / 2.14e-3,
-// rank 16 plus 5 % noise 700 x 2816 1.76 / 1.83e-3; none / first: 256 x 512 1.94 / 1.94e-3: the first pair costs
-// nothing, the second little where m is large.  On the GPU, the worst of 35 normal 640 x 1280: 2.51e-3 with both.
+// How many of the leading pairs of steps, (0, 1) and (2, 3), run as one product with X.  Each saves 3 m^2 (n - m)
+// operations, costs 2 m^3 and a stage, and moves X's planes once less.
+// Speed, in us without / with: first pair, n = 1.5 m, 204 of 256 x 384 347 / 329, 51 of 512 x 768 331 / 320, 33 of
+// 640 x 960 382 / 379, 2048 x 3072 288 / 296; n = 2 m, 10 of 1024 x 2048 430 / 414, 4096 x 8192 2109 / 2040; two matrices alone
+// take 2 to 4 us more.  Second pair, n = 2 m, 25 of 640 x 1280 359 / 356, 10 of 1024 x 2048 414 / 411, 2048 x 4096 343 / 339,
+// 4096 x 8192 2040 / 1933; n = 2.5 m, 20 of 640 x 1600 351 / 333, 4096 x 10240 2371 / 2286.
+// Relative error against 64-bit results with none / the first / both (1.66e-3 is rounding them to bf16): normal
+// elements, 640 x 1920 1.81 / 1.81 / 2.19e-3, but both 2.33e-3 at 512 x 1280: hence 640; rank 32, 1024 x 4096 3.05 / 3.08 / 4.92e-3;
+// rank 1 3.76 / 4.08 / 4.68e-3.
 int pairs(int64_t m, int64_t n, const float* coef, int steps) {
   int count = 0;
   double top = 1.0;  // bound of the singular values before step s
   for (int s = 0; s + 2 <= steps && s < 4; s += 2) {
-    const bool worth = s == 0 ? n * 2 >= m * 3 && m >= 256 : n >= m * 2 && m >= (n >= m * 3 ? 640 : 768);
+    const bool worth = s == 0 ? m >= 256 && (n >= m * 2 || (m <= 512 && n * 2 >= m * 3))
+                              : m >= 640 && (n * 2 >= m * 5 || (m >= 2048 && n >= m * 2));
     const double between = ns_growth(coef + 3 * s, top);
     // both factors' product has to fit the planes like each of them
     if (!worth || ns_factor(coef + 3 * s, top) * ns_factor(coef + 3 * s + 3, between) > kMaxFactor) break;
@@ -764,9 +774,10 @@ int make_stages(NsBatch* shape, const float* coef, int steps, int map0, int coun
     g.diagonal_all = int(b.m_pad * b.n);
     return &g;
   };
-  // a symmetric m x m product of square matrices x and y, which commute
-  auto multiply = [&](Epilogue e, int x, int y, int to) {
+  // x y^T of square matrices x and y; `mirror`: it is symmetric
+  auto multiply = [&](Epilogue e, int x, int y, int to, bool mirror) {
     Stage* g = add(e, m, m, m);
+    g->mirror = mirror;
     g->map_a = uint8_t(map0 + kMapSq + x);
     g->map_b = uint8_t(map0 + kMapSq + y);
     g->map_out = uint8_t(map0 + kMapSqOut + to);
@@ -779,7 +790,7 @@ int make_stages(NsBatch* shape, const float* coef, int steps, int map0, int coun
     return g;
   };
   auto factor = [&](int gram, int to, const float* c) {  // c0 I + c1 G + c2 G G
-    Stage* g = multiply(kPoly, gram, gram, to);
+    Stage* g = multiply(kPoly, gram, gram, to, true);
     g->scale = c[2] / kScaleG;
     g->add = c[1];
     g->diag = c[0] * kScaleG;
@@ -789,7 +800,8 @@ int make_stages(NsBatch* shape, const float* coef, int steps, int map0, int coun
   for (int s = 0; s < steps;) {
     const bool pair = s < 2 * merged;
     const float* c = coef + 3 * s;
-    Stage* g = add(kSymmetric, m, m, n);
+    Stage* g = add(kSquare, m, m, n);
+    g->mirror = true;
     g->a_mn = g->b_mn = tall;
     g->map_a = g->map_b = uint8_t(map0 + (tall ? kMapXmn : kMapXk) + cur);
     g->map_out = uint8_t(map0 + kMapSqOut);
@@ -798,10 +810,10 @@ int make_stages(NsBatch* shape, const float* coef, int steps, int map0, int coun
     g->scale = kScaleG / (kScaleX * kScaleX);
     factor(0, 1, c);
     if (pair) {
-      multiply(kSymmetric, 0, 1, 2);
-      multiply(kSymmetric, 2, 1, 0);  // G' = G Q1 Q1
+      multiply(kSquare, 1, 0, 2, false);  // Q1 G
+      multiply(kSquare, 1, 2, 0, true);   // G' = Q1 (Q1 G)^T
       factor(0, 2, c + 3);
-      multiply(kSymmetric, 2, 1, 0);  // Q2 Q1
+      multiply(kSquare, 2, 1, 0, false);  // Q2 Q1
     }
     const int q = pair ? 0 : 1;
     g = add(s < kPreciseSteps ? kPrecise : kPlain, int(b.rows), int(b.cols), m);
@@ -848,7 +860,7 @@ bool cut(Stage* stages, int count, int64_t batch, int cg, int workers, double* w
     Stage& g = stages[s];
     g.tiles_m = (g.M + tile - 1) / tile;
     g.tiles_n = (g.N + tile - 1) / tile;
-    const int64_t per = g.epilogue <= kPoly ? int64_t(g.tiles_m) * (g.tiles_m + 1) / 2 : int64_t(g.tiles_m) * g.tiles_n;
+    const int64_t per = g.mirror ? int64_t(g.tiles_m) * (g.tiles_m + 1) / 2 : int64_t(g.tiles_m) * g.tiles_n;
     if (per * batch > 0x3fffffff || before > 0x7fffffff) return false;
     g.per_matrix = int(per);
     g.m_fast = g.tiles_m <= g.tiles_n;  // the shorter side first: its operand panels stay in L2
