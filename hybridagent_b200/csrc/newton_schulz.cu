@@ -10,7 +10,10 @@
 //
 // Rounding X itself is what a strongly graded spectrum is sensitive to: the rounding noise of the
 // leading directions is full-rank and is amplified as much as the small singular values (485-fold
-// in five steps).  So the first kPreciseSteps steps keep X as a high and a low fp16 plane (22 bits).
+// in five steps).  So X is kept as a high and a low fp16 plane (22 bits) until the steps that are left multiply by
+// no more than kPlainGain: in all but the last two of the usual steps, however many there are.  With a low plane in the
+// first three steps only, 300 x 400 of rank 4 was off by 8e-3 after six steps, 0.1 after eight and 1.1 after ten; now by 3e-3,
+// 6e-3 and 6e-2, which is what the accumulators cut off (2^-21 of X in a step), multiplied by 3.44 in every later step.
 // The products read the high plane only: with a on B's diagonal a step is (a I + B) X, and its
 // epilogue adds a * low in fp32 (what B does to the low plane touches only the few leading
 // directions).  Against 64-bit results (rank-16 plus 5 % noise, 1024 x 1024, rounded to bf16): 2.1e-3
@@ -67,7 +70,8 @@ namespace {
 constexpr int kBM = 128;           // rows of a CTA's part of a tile: the TMEM lanes
 constexpr int kBK = 64;            // K elements of a ring slot: one 128-byte swizzle row
 constexpr int kGemmThreads = 416;  // operands, MMA, addends, stores; eight epilogue warps; stores
-constexpr int kPreciseSteps = 3;
+constexpr int kPreciseSteps = 3;   // with a low plane of X in any case
+constexpr double kPlainGain = 12;  // of the steps that a single plane's rounding may go through (3.4445^2 is 11.9)
 constexpr int kHalf = kBM * kBK * 2;  // bytes of one operand's part of a slot
 constexpr int kSlot = 2 * kHalf;
 constexpr int kSlots = 5;
@@ -796,6 +800,14 @@ int make_stages(NsBatch* shape, const float* coef, int steps, int map0, int coun
     g->diag = c[0] * kScaleG;
   };
   const int merged = pairs(m, n, coef, steps);
+  double left[HA_NS_MAX_STEPS + 1], top = 1.0;  // what steps s .. multiply by at most
+  for (int s = 0; s < steps; ++s) {
+    left[s] = ns_factor(coef + 3 * s, top);
+    top = ns_growth(coef + 3 * s, top);
+  }
+  left[steps] = 1.0;
+  for (int s = steps; s-- > 0;) left[s] = left[s + 1] * (left[s] > 1.0 ? left[s] : 1.0);
+  auto low_before = [&](int s) { return s < steps && (s < kPreciseSteps || left[s] > kPlainGain); };
   int cur = 0;
   for (int s = 0; s < steps;) {
     const bool pair = s < 2 * merged;
@@ -816,7 +828,7 @@ int make_stages(NsBatch* shape, const float* coef, int steps, int map0, int coun
       multiply(kSquare, 2, 1, 0, false);  // Q2 Q1
     }
     const int q = pair ? 0 : 1;
-    g = add(s < kPreciseSteps ? kPrecise : kPlain, int(b.rows), int(b.cols), m);
+    g = add(low_before(s) ? kPrecise : kPlain, int(b.rows), int(b.cols), m);
     g->b_mn = !tall;
     g->by_column = tall;
     g->square_1 = int8_t(q);
@@ -828,7 +840,7 @@ int make_stages(NsBatch* shape, const float* coef, int steps, int map0, int coun
     g->scale = 1.0f / kScaleG;
     g->add = (pair ? c[0] * c[3] : c[0]) / kScaleLo;
     s += pair ? 2 : 1;
-    g->keep_low = s < kPreciseSteps && s < steps;  // the next step reads it
+    g->keep_low = low_before(s);  // the next step reads it
   }
   Stage& last = stages[count - 1];
   shape->out = cur;
