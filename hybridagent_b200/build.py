@@ -41,7 +41,7 @@ def _nccl_include() -> str:
 def _sources() -> list[str]:
     files = [os.path.join(CSRC, f) for f in CU_SOURCES + CPP_SOURCES]
     files += [os.path.join(CSRC, "ha_common.cuh"), os.path.join(CSRC, "ha_nvtx.h"),
-              *(os.path.join(CSRC, f) for f in ("ha_param.cuh", "umma.cuh", "newton_schulz.cuh")),
+              *(os.path.join(CSRC, f) for f in ("ha_param.cuh", "bounded_wait.h", "umma.cuh", "newton_schulz.cuh")),
               os.path.join(INCLUDE, "hybridagent_b200.h"), __file__]
     return files
 

@@ -142,9 +142,13 @@ __global__ void __launch_bounds__(kThreadsN, 1) narrow_kernel(const __grid_const
   grid_wait();  // the load kernel's planes
   const uint32_t tmem = tmem_s, lanes = tmem + (uint32_t(quarter * 32) << 16);
   uint32_t done_phase = 0;  // bit i: phase of bars.done[i]
+  // Once a wait has run out the pieces that are left are left undone, in this part and in all that follow; the barriers of
+  // the CTA and of the cluster are gone through all the same.
+  bool ok = true;      // no wait of this thread has run out
+  bool dead = false;   // one of the CTA's has, in an earlier part
   auto wait_done = [&](int i) {
     __syncwarp();
-    mbar_wait(smem_u32(&bars.done[i]), (done_phase >> i) & 1, &stop);
+    ok &= mbar_wait<true>(smem_u32(&bars.done[i]), (done_phase >> i) & 1, &stop);
     __syncwarp();  // lanes leave the polling loop one by one; TMEM reads and barriers need the whole warp
     done_phase ^= 1u << i;
     tc_fence_after();
@@ -175,7 +179,7 @@ __global__ void __launch_bounds__(kThreadsN, 1) narrow_kernel(const __grid_const
 
   auto wait_full = [&](int slot) {
     __syncwarp();
-    mbar_wait(smem_u32(&bars.full[slot]), (full_phase >> slot) & 1, &stop);
+    ok &= mbar_wait<true>(smem_u32(&bars.full[slot]), (full_phase >> slot) & 1, &stop);
     __syncwarp();
     full_phase ^= 1u << slot;
     tc_fence_after();
@@ -186,14 +190,16 @@ __global__ void __launch_bounds__(kThreadsN, 1) narrow_kernel(const __grid_const
   while (!((p.ends >> (s1 - 1)) & 1)) ++s1;
   // ---- G: high x high into columns 0.., the cross terms (2^11 larger) into columns 128..
   const int gram_slots = nblk == 2 ? 3 : kRing;
+  const int gram_pieces = dead ? 0 : pieces;
   if (warp == 0) {
     const uint32_t idesc = f16_idesc(128, np, p.tall, p.tall);
     const int ksteps = span / 16;
-    for (int i = 0; i < min(pieces, gram_slots); ++i)
+    for (int i = 0; i < min(gram_pieces, gram_slots); ++i)
       if (elect_one()) load_piece(i, base + i * piece_bytes, smem_u32(&bars.full[i]));
-    for (int i = 0; i < pieces; ++i) {
+    for (int i = 0; i < gram_pieces; ++i) {
       const int slot = i % gram_slots;
       wait_full(slot);
+      if (!__all_sync(0xffffffffu, ok)) break;
       const uint32_t hi = base + slot * piece_bytes, lo = hi + piece_bytes / 2;
       if (elect_one()) {
         const uint32_t h = smem_desc(hi, kHalfPlane), l = smem_desc(lo, kHalfPlane);
@@ -204,9 +210,9 @@ __global__ void __launch_bounds__(kThreadsN, 1) narrow_kernel(const __grid_const
         mma_commit<1>(smem_u32(&bars.empty[slot]));
       }
       emptied ^= 1u << slot;
-      if (i + gram_slots < pieces) {
+      if (i + gram_slots < gram_pieces) {
         __syncwarp();
-        mbar_wait(smem_u32(&bars.empty[slot]), ((emptied >> slot) & 1) ^ 1, &stop);
+        ok &= mbar_wait<true>(smem_u32(&bars.empty[slot]), ((emptied >> slot) & 1) ^ 1, &stop);
         __syncwarp();
         if (elect_one()) load_piece(i + gram_slots, base + slot * piece_bytes, smem_u32(&bars.full[slot]));
       }
@@ -225,7 +231,7 @@ __global__ void __launch_bounds__(kThreadsN, 1) narrow_kernel(const __grid_const
       float x[32];
 #pragma unroll
       for (int j = 0; j < 32; ++j)
-        x[j] = pieces == 0 ? 0.0f
+        x[j] = gram_pieces == 0 ? 0.0f
                            : __fmaf_rn(__uint_as_float(b[j]), 1.0f / kScaleLo, __uint_as_float(a[j])) *
                                  (kScaleN / (kScaleX * kScaleX));
       if (row < np) {
@@ -381,6 +387,7 @@ __global__ void __launch_bounds__(kThreadsN, 1) narrow_kernel(const __grid_const
   const uint32_t ring = base + kOffG, staging = base + kBytes - stages * 2 * kHalfPlane;
   const bool idle = quarter * 32 >= (p.tall ? 128 : np);            // no row of this warp is stored
   int stored = 0;
+  const int todo = __syncthreads_or(int(stop)) ? 0 : pieces;
   const uint32_t idesc = p.tall ? f16_idesc(128, np, false, false) : f16_idesc(128, 64, false, true);
   const bool both = s1 < p.steps;  // X goes on: high and low plane
   const bool bf16 = p.bf16 && !both, direct = p.direct && !both;
@@ -408,15 +415,16 @@ __global__ void __launch_bounds__(kThreadsN, 1) narrow_kernel(const __grid_const
     mma_commit<1>(smem_u32(&bars.done[i & 1]));
   };
   if (warp == 0) {
-    for (int i = 0; i < min(pieces, slots); ++i)
+    for (int i = 0; i < min(todo, slots); ++i)
       if (elect_one()) load_piece(i, ring + i * piece_bytes, smem_u32(&bars.full[i]));
-    if (pieces > 0) issue(0);
+    if (todo > 0) issue(0);
   }
-  for (int i = 0; i < pieces; ++i) {
-    if (warp == 0 && i + 1 < pieces) issue(i + 1);
+  for (int i = 0; i < todo; ++i) {
+    if ((i & 31) == 31 && __syncthreads_or(int(stop))) break;  // (every time: 5 % of 64 of 32 x 4096)
+    if (warp == 0 && i + 1 < todo) issue(i + 1);
     __syncwarp();
     wait_done(i & 1);
-    if (warp == 0 && i + slots < pieces && elect_one())  // piece i's slot has been read
+    if (warp == 0 && i + slots < todo && elect_one() && ok)  // piece i's slot has been read
       load_piece(i + slots, ring + (i % slots) * piece_bytes, smem_u32(&bars.full[i % slots]));
     for (int blk = 0; blk < nblk; ++blk, ++stored) {  // 64 columns at a time: 32 for each half of the warps
       if (stages == 1) {
@@ -468,11 +476,11 @@ __global__ void __launch_bounds__(kThreadsN, 1) narrow_kernel(const __grid_const
     }
   }
   if (warp == 0 && elect_one()) tma_store_wait_all();  // this CTA reads back only what it stored itself
-  __syncthreads();
+  dead = __syncthreads_or(int(stop));
   plane ^= 1;
   s0 = s1;
   }
-  if (stop) {  // a wait ran out: let copies and products in flight end before their memory is given up
+  if (dead) {  // a wait ran out: let copies and products in flight end before their memory is given up
     if (threadIdx.x == 0) atomicExch(p.error, 1u);
     const uint64_t t0 = global_ns();
     while (global_ns() - t0 < 2000000) {

@@ -8,6 +8,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include "bounded_wait.h"
+
 namespace ha {
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {
@@ -77,23 +79,12 @@ __device__ __forceinline__ void grid_launch_dependents() {
 }
 __device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
-// Bounded wait: false once `kWaitNs` have passed, or as soon as another thread of the CTA gave up
-// (*stop).  No wait of a healthy launch comes near the limit: it is some hundred times the longest
-// kernel; it turns a lost arrival into an error word instead of a GPU that never answers.
+// A bounded wait (bounded_wait.h).  No wait of a healthy launch comes near the limit: it is some hundred times the
+// longest kernel; it turns a lost arrival into an error word instead of a GPU that never answers.
 constexpr uint64_t kWaitNs = 4000000000ull;
+template <bool EARLY = false>
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile uint32_t* stop) {
-  if (mbar_try(bar, parity)) return true;
-  const uint64_t t0 = global_ns();
-  for (;;) {
-#pragma unroll 1
-    for (int i = 0; i < 256; ++i)
-      if (mbar_try(bar, parity)) return true;
-    if (*stop) return false;
-    if (global_ns() - t0 > kWaitNs) {
-      *stop = 1;
-      return false;
-    }
-  }
+  return bounded_wait<EARLY>([&] { return mbar_try(bar, parity); }, [] { return global_ns(); }, stop, kWaitNs);
 }
 
 // The same for a counter in global memory that other CTAs of the launch raise: true once it has
@@ -104,20 +95,7 @@ __device__ __forceinline__ uint32_t load_acquire(const uint32_t* p) {
   return v;
 }
 __device__ __forceinline__ bool counter_wait(const uint32_t* counter, uint32_t want, volatile uint32_t* stop) {
-  if (load_acquire(counter) < want) {
-    const uint64_t t0 = global_ns();
-    for (;;) {
-      bool done = false;
-#pragma unroll 1
-      for (int i = 0; i < 256 && !done; ++i) done = load_acquire(counter) >= want;
-      if (done) break;
-      if (*stop) return false;
-      if (global_ns() - t0 > kWaitNs) {
-        *stop = 1;
-        return false;
-      }
-    }
-  }
+  if (!bounded_wait<false>([&] { return load_acquire(counter) >= want; }, [] { return global_ns(); }, stop, kWaitNs)) return false;
   asm volatile("fence.proxy.async;" ::: "memory");
   return true;
 }
@@ -131,17 +109,7 @@ __device__ __forceinline__ uint32_t granted_now(uint32_t* granted) {
   return v;
 }
 __device__ __forceinline__ bool granted_wait(uint32_t* granted, uint32_t want, volatile uint32_t* stop) {
-  const uint64_t t0 = global_ns();
-  for (uint32_t i = 1;; ++i) {
-    if (granted_now(granted) >= want) break;
-    if ((i & 255) == 0) {
-      if (*stop) return false;
-      if (global_ns() - t0 > kWaitNs) {
-        *stop = 1;
-        return false;
-      }
-    }
-  }
+  if (!bounded_wait<false>([&] { return granted_now(granted) >= want; }, [] { return global_ns(); }, stop, kWaitNs)) return false;
   asm volatile("fence.proxy.async;" ::: "memory");
   return true;
 }
