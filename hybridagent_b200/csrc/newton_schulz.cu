@@ -622,6 +622,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) newton_schulz_kernel(const __
     if (lane == 0) {
       store_blocks<CG>(p, sh, ring + kSlots * kSlot, walk, int(rank), warp == 3 ? 0 : 1);
       tma_store_wait_all();
+      if (p.dst != nullptr && any_gave_up(p.error)) sh.stop = 1;
     }
     __syncwarp();
   } else {
@@ -649,12 +650,12 @@ __global__ void __launch_bounds__(kGemmThreads, 1) newton_schulz_kernel(const __
   }
   __syncthreads();
   if (sh.stop) {  // a wait ran out: let copies and products in flight end before their memory is given up
-    if (threadIdx.x == 0) atomicExch(p.error, 1u);
+    if (threadIdx.x == 0) gave_up(p.error);
     const uint64_t t0 = global_ns();
     while (global_ns() - t0 < 2000000) {
     }
-    if (p.dst != nullptr)
-      for (int64_t e = threadIdx.x; e < p.dst_elems; e += kGemmThreads) p.dst[e] = 0x7fff;
+    __syncthreads();
+    if (p.dst != nullptr) fill_nan(p.dst, p.dst_elems, kGemmThreads);
     __syncthreads();
   }
   tc_fence_before();

@@ -475,18 +475,21 @@ __global__ void __launch_bounds__(kThreadsN, 1) narrow_kernel(const __grid_const
       __syncwarp();
     }
   }
-  if (warp == 0 && elect_one()) tma_store_wait_all();  // this CTA reads back only what it stored itself
+  if (warp == 0 && elect_one()) {
+    tma_store_wait_all();  // this CTA reads back only what it stored itself
+    if (direct && any_gave_up(p.error)) stop = 1;
+  }
   dead = __syncthreads_or(int(stop));
   plane ^= 1;
   s0 = s1;
   }
   if (dead) {  // a wait ran out: let copies and products in flight end before their memory is given up
-    if (threadIdx.x == 0) atomicExch(p.error, 1u);
+    if (threadIdx.x == 0) gave_up(p.error);
     const uint64_t t0 = global_ns();
     while (global_ns() - t0 < 2000000) {
     }
-    if (p.direct)
-      for (int64_t e = threadIdx.x; e < p.out_elems; e += kThreadsN) p.out[e] = 0x7fff;
+    __syncthreads();
+    if (p.direct) fill_nan(p.out, p.out_elems, kThreadsN);
   }
   tc_fence_before();
   __syncthreads();

@@ -118,6 +118,25 @@ __device__ __forceinline__ void counter_raise(uint32_t* counter) {
   asm volatile("red.release.gpu.global.add.u32 [%0], 1;" ::"l"(counter) : "memory");
 }
 
+// ---------------------------------------------------------------- launches that gave up
+// Whether a CTA of this launch, or of one before it, gave up, asked by a thread whose stores have completed.  Either the
+// answer is yes, or those stores lie before whatever a CTA writes after gave_up(): so the result of a launch that all
+// CTAs end with this, and with fill_nan() if it says yes, is NaN as a whole or right.
+__device__ __forceinline__ bool any_gave_up(const uint32_t* error) {
+  __threadfence();
+  return load_acquire(error) != 0;
+}
+// One thread of a CTA that gave up.
+__device__ __forceinline__ void gave_up(uint32_t* error) {
+  atomicExch(error, 1u);
+  __threadfence();
+}
+// All `threads` threads of a CTA, after a barrier; dst is 16-byte aligned, elems a multiple of 8.
+__device__ __forceinline__ void fill_nan(uint16_t* dst, int64_t elems, int threads) {
+  const uint4 nan = make_uint4(0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu);
+  for (int64_t e = int64_t(threadIdx.x) * 8; e < elems; e += int64_t(threads) * 8) *reinterpret_cast<uint4*>(dst + e) = nan;
+}
+
 // ---------------------------------------------------------------- TMA
 __device__ __forceinline__ void tma_prefetch_map(const CUtensorMap* map) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");

@@ -281,7 +281,8 @@ int ha_orthogonalize_workspace(int64_t batch, int64_t rows, int64_t cols, size_t
 /* Orthogonalises `batch` contiguous row-major matrices of rows x cols: singular values towards 1, singular
  * vectors kept.  src holds src_dtype (HA_F32 / HA_BF16 / HA_F16), dst receives bf16.  src and dst may
  * not overlap.  A non-finite element makes its matrix NaN.  workspace: device memory, 256-byte aligned, not
- * shared with a call that may run at the same time.  Should a wait inside the products run out, dst is NaN. */
+ * shared with a call that may run at the same time.  Should a wait inside the products run out, all matrices of that pass
+ * through the workspace and of later ones are NaN. */
 int ha_orthogonalize(const void* src, int src_dtype, void* dst, int64_t batch, int64_t rows, int64_t cols,
                      const ha_ns_params* ns, void* workspace, size_t workspace_bytes, void* stream);
 
