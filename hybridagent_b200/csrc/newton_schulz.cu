@@ -266,9 +266,7 @@ __device__ __forceinline__ bool epilogue(const Stage& g, const Job& job, Warp& w
     ++w.tile;
     if (wanted(at)) {
       if (!fetched) {
-        bool ok = true;
-        if (lane == 0) ok = granted_wait(&sh.granted, w.tile, &sh.stop);
-        if (!__all_sync(0xffffffffu, ok)) return false;
+        if (!granted_wait_warp(&sh.granted, w.tile, &sh.stop, lane)) return false;
         fetch(at, k0);
       }
       if (kSym) {
@@ -285,7 +283,7 @@ __device__ __forceinline__ bool epilogue(const Stage& g, const Job& job, Warp& w
     fetched = false;
     if (t + w.walk.step < tiles) {
       const TileAt next = tile_at(g, t + w.walk.step);
-      if (wanted(next) && __all_sync(0xffffffffu, lane != 0 || granted_now(&sh.granted) > w.tile)) {
+      if (wanted(next) && granted_to_warp(&sh.granted, w.tile + 1, lane)) {
         fetch(next, k0 ^ (blocks & 1));
         fetched = true;
       }

@@ -113,6 +113,18 @@ __device__ __forceinline__ bool granted_wait(uint32_t* granted, uint32_t want, v
   asm volatile("fence.proxy.async;" ::: "memory");
   return true;
 }
+// The same for all lanes of a converged warp: lane 0 looks or waits, and what it has acquired is ordered before what the
+// others read afterwards by __syncwarp() (a vote orders no memory).
+__device__ __forceinline__ bool granted_to_warp(uint32_t* granted, uint32_t want, int lane) {
+  const bool yes = __all_sync(0xffffffffu, lane != 0 || granted_now(granted) >= want);
+  __syncwarp();
+  return yes;
+}
+__device__ __forceinline__ bool granted_wait_warp(uint32_t* granted, uint32_t want, volatile uint32_t* stop, int lane) {
+  const bool yes = __all_sync(0xffffffffu, lane != 0 || granted_wait(granted, want, stop));
+  __syncwarp();
+  return yes;
+}
 // Raises it after this thread's TMA stores, which have completed.
 __device__ __forceinline__ void counter_raise(uint32_t* counter) {
   asm volatile("red.release.gpu.global.add.u32 [%0], 1;" ::"l"(counter) : "memory");

@@ -77,6 +77,19 @@ def test_the_flag_ends_it_at_the_next_look(lines):
     assert lines["late"][7] == lines["early"][7] == (0, 1 + 3 * 256, 1)  # set before try 700
 
 
+def test_warps_read_behind_a_barrier_what_one_lane_has_acquired():
+    """The epilogue warps read diagonals that other CTAs stored after lane 0 alone has acquired the word that says so."""
+    umma = open(os.path.join(CSRC, "umma.cuh")).read()
+    for name in ("granted_to_warp(", "granted_wait_warp("):
+        at = umma.index(name)
+        body = umma[at:umma.index("\n}\n", at)]
+        assert body.index("__all_sync(") < body.index("__syncwarp();") < body.index("return yes;")
+    wide = open(os.path.join(CSRC, "newton_schulz.cu")).read()
+    assert "granted_now(" not in wide
+    for at in (m.start() for m in re.finditer("granted_wait\\(", wide)):  # by single threads, for what they copy
+        assert "Warp" not in wide[wide.rindex("\ntemplate", 0, at):at].split("{")[0]
+
+
 def test_every_wait_of_the_kernels_is_this_one():
     """No kernel polls a barrier by itself.  The narrow one, whose barriers keep all of its threads to the end, takes each
     wait's result and leaves the loops over a matrix's pieces, of which there may be thousands."""
