@@ -199,7 +199,6 @@ class ZeroOneMuon(ZeroOneAdamW):
 
     def _update_muon(self, c, sc: _lib.AdamwScalars, changed_only: bool, p2p: bool) -> None:
         """The Muon update of class c's owned matrices that have a gradient."""
-        self._check_status()
         ms = _lib.MuonScalars(np.float32(self.momentum), np.float32(1.0 - self.momentum), int(self.nesterov),
                               sc.use_decay, sc.clip, sc.clip_mult)
         table = np.ascontiguousarray(c.table.np[c.order])
@@ -214,13 +213,25 @@ class ZeroOneMuon(ZeroOneAdamW):
     def _check_status(self) -> None:
         """Raises if the products of a step that has run gave up."""
         if int(self._muon_status[0]) != 0:
-            raise RuntimeError("Muon step: a wait inside the Newton-Schulz products ran out; the matrices of that "
-                               "step were not updated")
+            raise RuntimeError("Muon step: a wait inside the Newton-Schulz products of an earlier step ran out.  Matrices of "
+                               "that step kept their weights (all but those of passes through the workspace that were "
+                               "done before), while momenta, step counts and other tensors advanced: load a checkpoint "
+                               "(load_state_dict) to go on")
+
+    def step(self) -> None:
+        """``ZeroOneAdamW.step`` with Muon's update of the matrices.  Raises, before anything changes, if the products of an
+        earlier step are known to have given up."""
+        self._check_status()
+        super().step()
 
     def state_dict(self) -> dict:
         state = super().state_dict()  # (waits for the steps before)
         self._check_status()
         return state
+
+    def load_state_dict(self, state: dict) -> None:
+        super().load_state_dict(state)  # (waits for the steps before)
+        self._muon_status.zero_()
 
     def state_summary(self) -> str:
         n = sum(len(c.layout.indices) for c in self._classes if c.muon)

@@ -294,7 +294,8 @@ int ha_orthogonalize(const void* src, int src_dtype, void* dst, int64_t batch, i
  * the master is the parameter).  exp_avg_sq, rc1 and rc2 are not read; neg_lr includes any factor for
  * the shape.  changed_only: 16-bit copies are stored by changed sectors, under ha_adamw_step_delta's
  * conditions; peers (may be NULL) and d_changed_groups as there.  Should a wait inside the products
- * run out, the weights stay as they are and *d_status (device or pinned host memory, may be NULL) becomes 1. */
+ * run out, momenta have advanced, the weights of that pass through the workspace and of later ones stay as they are, and
+ * *d_status (device or pinned host memory, may be NULL) becomes 1. */
 int ha_muon_step(const ha_tensor* h_tensors, const int64_t* h_shapes, int64_t n, int grad_dtype,
                  const ha_muon_scalars* sc, const ha_ns_params* ns, int changed_only, const ha_peers* peers,
                  unsigned long long* d_changed_groups, uint32_t* d_status, void* workspace, size_t workspace_bytes,

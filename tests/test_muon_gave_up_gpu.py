@@ -104,3 +104,39 @@ def test_a_step_leaves_the_weights_and_sets_the_status(rows, cols):
         assert int(status) == 1
         assert torch.equal(master, before[0]) and torch.equal(param, before[1])
         assert moment.abs().max() > 0  # the momentum has been updated
+
+
+def test_the_optimizer_raises_before_anything_changes_until_a_state_is_loaded():
+    import torch
+    from hybridagent_b200 import ZeroOneMuon
+    gen = torch.Generator(device="cuda").manual_seed(0)
+    params = [torch.nn.Parameter(torch.randn(s, generator=gen, device="cuda").bfloat16()) for s in [(40, 60), (300, 280), (99,)]]
+    opt = ZeroOneMuon([{"params": params, "lr": 1e-2}], rank=0, world_size=1)
+
+    def grads():
+        for p in params:
+            p.grad = torch.randn(p.shape, generator=gen, device="cuda").bfloat16()
+
+    grads()
+    opt.clip_grad_norm(1.0)
+    opt.step()
+    good = opt.state_dict()
+    grads()
+    opt.clip_grad_norm(0.5)
+    opt._muon_status[0] = 1  # as the weights' kernel writes it
+    counts, clip = dict(opt.param_steps), opt._pending_clip
+    weights, moments = [p.detach().clone() for p in params], [opt.exp_avg[i].clone() for i in range(3)]
+    for _ in range(2):
+        with pytest.raises(RuntimeError, match="ran out"):
+            opt.step()
+        assert opt.step_count == 1 and dict(opt.param_steps) == counts and opt._pending_clip == clip is not None
+    with pytest.raises(RuntimeError, match="ran out"):
+        opt.state_dict()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(weights, params))
+    assert all(torch.equal(m, opt.exp_avg[i]) for i, m in enumerate(moments))
+    opt.load_state_dict(good)
+    grads()
+    opt.clip_grad_norm(1.0)
+    opt.step()
+    assert opt.state_dict()["step_count"] == 2
