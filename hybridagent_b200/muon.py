@@ -78,6 +78,17 @@ def _budget(name: str, default: int) -> int:
     return value
 
 
+def _workspace(size: int, least: int, device: torch.device) -> torch.Tensor:
+    """`size` bytes on `device`, or half of it, a quarter, ... but `least`, where memory is short."""
+    while True:
+        try:
+            return torch.empty(size, dtype=torch.uint8, device=device)
+        except torch.OutOfMemoryError:
+            if size <= least:
+                raise
+            size = max(size // 2, least)
+
+
 def orthogonalize(x: torch.Tensor, *, steps: int = 5, coefficients=COEFFICIENTS, eps: float = 1e-7,
                   out: torch.Tensor | None = None) -> torch.Tensor:
     """The Newton-Schulz orthogonalisation of ``x`` (..., rows, cols), each matrix for itself, as bf16.
@@ -87,7 +98,8 @@ def orthogonalize(x: torch.Tensor, *, steps: int = 5, coefficients=COEFFICIENTS,
     is divided by its Frobenius norm, or by ``eps`` where that is larger, so a zero matrix stays zero.
     One with a non-finite element becomes NaN.  Not differentiable.  Runs on the current stream of x's
     device without waiting for it and may be captured into a CUDA graph; temporary memory of up to
-    HYBRIDAGENT_B200_NS_BYTES (default 8 GiB; at least one matrix's planes) comes from torch."""
+    HYBRIDAGENT_B200_NS_BYTES (default 8 GiB; at least one matrix's planes) comes from torch, less where that much is
+    not free."""
     if not isinstance(x, torch.Tensor):
         raise TypeError(f"expected a tensor, got {type(x).__name__}")
     if x.dtype not in _CODES:
@@ -117,14 +129,14 @@ def orthogonalize(x: torch.Tensor, *, steps: int = 5, coefficients=COEFFICIENTS,
     if src.numel() == 0:
         return out
     batch = src.numel() // (rows * cols)
-    size = _workspace_bytes(batch, rows, cols)
+    size, least = _workspace_bytes(batch, rows, cols), _workspace_bytes(1, rows, cols)
     budget = _budget("HYBRIDAGENT_B200_NS_BYTES", 8 << 30)
     if size > budget:
-        size = min(size, max(budget, _workspace_bytes(1, rows, cols)))
-    ws = torch.empty(size, dtype=torch.uint8, device=x.device)
+        size = max(budget, least)
+    ws = _workspace(size, least, x.device)
     device = x.device.index
     args = ("ha_orthogonalize", src.data_ptr(), _CODES[x.dtype], out.data_ptr(), batch, rows, cols, ctypes.byref(ns),
-            ws.data_ptr(), size, torch._C._cuda_getCurrentRawStream(device))
+            ws.data_ptr(), ws.numel(), torch._C._cuda_getCurrentRawStream(device))
     if device == torch._C._cuda_getDevice():
         _lib.call(*args)
     else:
@@ -146,7 +158,7 @@ class ZeroOneMuon(ZeroOneAdamW):
     ``"use_muon": False``.  ``betas`` and ``eps`` belong to the AdamW tensors, ``weight_decay`` to both.
     ``exp_avg`` holds a Muon tensor's momentum; it has no ``exp_avg_sq``.  Workspace for the products, of
     HYBRIDAGENT_B200_MUON_BYTES (default 4 GiB, at least the largest owned matrix's need and no more than
-    all of them need), is held for the optimizer's life."""
+    all of them need; less where that much is not free), is held for the optimizer's life."""
 
     state_format = "hybridagent_b200.zero1_muon/1"
     _updates = ("AdamW", "Muon")
@@ -167,17 +179,18 @@ class ZeroOneMuon(ZeroOneAdamW):
                          weight_decay=weight_decay, comm_timeout_s=comm_timeout_s, land_grads=land_grads)
         muon = [c for c in self._classes if c.muon and c.owned]
         with torch.cuda.device(self.device):
-            size, budget = 0, _budget("HYBRIDAGENT_B200_MUON_BYTES", 4 << 30)
+            size, least, budget = 0, 0, _budget("HYBRIDAGENT_B200_MUON_BYTES", 4 << 30)
             for c in muon:
                 shapes = [tuple(self.params[i].shape) for i in c.owned]
                 # equal shapes follow one another: they run together
                 c.order = np.asarray(sorted(range(len(shapes)), key=lambda k: shapes[k]), dtype=np.int64)
                 c.shapes = np.ascontiguousarray([shapes[k] for k in c.order], dtype=np.int64)
                 need = sum(_workspace_bytes(1, *s) for s in shapes)
-                size = max(size, min(need, max(budget, *(_workspace_bytes(1, *s) for s in set(shapes)), 0)))
+                least = max(least, *(_workspace_bytes(1, *s) for s in set(shapes)), 0)
+                size = max(size, min(need, max(budget, least)))
                 c.neg_lr = np.asarray([-(self.lrs[i] * self._factor(*self.params[i].shape)) for i in c.owned],
                                       dtype=np.float32)
-            self._muon_ws = torch.empty(size, dtype=torch.uint8, device=self.device) if size else None
+            self._muon_ws = _workspace(size, least, self.device) if size else None
             # set by a step whose products gave up; pinned host memory, which the GPU writes itself
             self._muon_status = torch.zeros(1, dtype=torch.int32, pin_memory=True)
             torch.cuda.current_stream().synchronize()
