@@ -93,7 +93,8 @@ def orthogonalize(x: torch.Tensor, *, steps: int = 5, coefficients=COEFFICIENTS,
                   out: torch.Tensor | None = None) -> torch.Tensor:
     """The Newton-Schulz orthogonalisation of ``x`` (..., rows, cols), each matrix for itself, as bf16.
 
-    ``x`` is fp32, bf16 or fp16 on a CUDA device; matrices that are not contiguous are copied first.
+    ``x`` is fp32, bf16 or fp16 on a CUDA device; matrices that are not contiguous are copied first, but for
+    transposed views of contiguous ones, whose result is such a view too unless ``out`` is given.
     ``out`` (bf16, contiguous, of x's shape, not overlapping it) receives the result if given.  A matrix
     is divided by its Frobenius norm, or by ``eps`` where that is larger, so a zero matrix stays zero.
     One with a non-finite element becomes NaN.  Not differentiable.  Runs on the current stream of x's
@@ -122,7 +123,8 @@ def orthogonalize(x: torch.Tensor, *, steps: int = 5, coefficients=COEFFICIENTS,
         return orthogonalize(x.mT, steps=steps, coefficients=coefficients, eps=eps).mT
     rows, cols = x.shape[-2:]
     src = x.contiguous()
-    if out is None:
+    given = out is not None
+    if not given:
         out = torch.empty(x.shape, dtype=torch.bfloat16, device=x.device)
     elif src is x and _overlap(x, out):
         raise ValueError("out overlaps x")
@@ -142,6 +144,8 @@ def orthogonalize(x: torch.Tensor, *, steps: int = 5, coefficients=COEFFICIENTS,
     else:
         with torch.cuda.device(device):
             _lib.call(*args)
+    if given:
+        torch.autograd.graph.increment_version(out)  # written through its address
     return out
 
 
