@@ -78,6 +78,10 @@ constexpr int kSlots = 5;
 constexpr int kBlockCols = 32;
 constexpr int kBlock = kBM * kBlockCols * 2;  // bytes of an epilogue block
 constexpr int kBlocks = 4;                    // in the ring, each with room for a second result
+// Gram matrices along more than 32768 are added up in parts of that.  The matrix unit cuts its sums off instead of rounding
+// them, about 2^-24 of the sum at each of K / 16 additions, always downwards: 160 x 524288 was off by 6.1e-3, 160 x 2097152 by
+// 2.3e-2.  A part's accumulators are added in fp32 to what the parts before left in the X plane that is free then.
+constexpr int kPartBlocks = 32768 / kBK;
 constexpr int kGemmSmem = kSlots * kSlot + kBlocks * 2 * kBlock + 1024;  // + alignment
 
 // What becomes of the accumulators (times `scale`):
@@ -114,6 +118,9 @@ struct Stage {
   int diagonal_each, diagonal_all;
   int8_t epilogue, m_fast, a_mn, b_mn, keep_low, by_column;  // *_mn: the operand's M / N index is the contiguous one
   int8_t mirror;        // D is symmetric
+  int part;             // blocks of K that are accumulated at once
+  float4* sums;         // of earlier parts: of matrix z at z * sums_each
+  int64_t sums_each;
 };
 // A stage of all `count` matrices of its shape.
 struct Job {
@@ -221,6 +228,61 @@ struct Warp {
   uint32_t acc, acc_phase;
 };
 
+// An epilogue warp's accumulators are read: the next products may use them.
+template <int CG>
+__device__ __forceinline__ void release_accumulator(Shared& sh, uint32_t acc, int lane) {
+  tc_fence_before();
+  __syncwarp();
+  if (lane == 0) {
+    const uint32_t bar = smem_u32(&sh.acc_empty[acc]);
+    if (CG == 2)
+      mbar_arrive_cluster(cluster_map(bar, 0));
+    else
+      mbar_arrive(bar);
+  }
+}
+
+// A tile whose products come in parts: adds up the accumulators of blocks k0, k0 + 2, .. in fp32, in `sums` (this lane's row
+// of block k, eight pieces of four columns 128 apart, at 1024 k), and leaves the sum in the last part's.  A thread reads
+// what it wrote itself.  (Not inline, and through TMEM: in the epilogue's code it cost every small matrix 2 to 4 us.)
+template <int CG>
+__device__ __noinline__ bool add_parts(Shared& sh, float4* sums, uint32_t tmem, uint32_t acc, uint32_t phase, int parts,
+                                       int k0, int blocks, int lane) {
+  for (int part = 1;; ++part) {
+    if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&sh.acc_full[acc]), phase, &sh.stop))) return false;
+    tc_fence_after();
+#pragma unroll 1
+    for (int k = k0; k < blocks; k += 2) {
+      const uint32_t from = tmem + acc * (128 * CG) + k * kBlockCols;
+      uint32_t v[32];
+      tmem_ld32(from, v);
+      tmem_ld_wait();
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        float4* at = sums + k * 1024 + j * 128;
+        float4 x = make_float4(__uint_as_float(v[4 * j]), __uint_as_float(v[4 * j + 1]), __uint_as_float(v[4 * j + 2]),
+                               __uint_as_float(v[4 * j + 3]));
+        if (part > 1) {
+          const float4 s = __ldcg(at);
+          x.x += s.x, x.y += s.y, x.z += s.z, x.w += s.w;
+        }
+        if (part < parts) __stcg(at, x);
+        v[4 * j] = __float_as_uint(x.x), v[4 * j + 1] = __float_as_uint(x.y);
+        v[4 * j + 2] = __float_as_uint(x.z), v[4 * j + 3] = __float_as_uint(x.w);
+      }
+      if (part == parts) tmem_st32(from, v);
+    }
+    if (part == parts) {
+      tmem_st_wait();
+      asm volatile("fence.proxy.async;" ::: "memory");  // the next product with X writes the sums' plane by TMA
+      return true;
+    }
+    release_accumulator<CG>(sh, acc, lane);
+    acc ^= 1;
+    phase ^= acc == 0;
+  }
+}
+
 template <int CG, int EPI>
 __device__ __forceinline__ bool epilogue(const Stage& g, const Job& job, Warp& w, Shared& sh) {
   constexpr bool kSym = EPI == kSquare || EPI == kPoly;
@@ -234,6 +296,7 @@ __device__ __forceinline__ bool epilogue(const Stage& g, const Job& job, Warp& w
   // Of the diagonals: (r, e) of this lane's row from both factors; factor of its row of X, or of its columns in
   // the group's blocks.
   float d[kSym ? 4 : 2 * CG];
+  const int parts = EPI == kSquare ? (g.K - 1) / kBK / g.part + 1 : 1;
   auto fetch = [&](const TileAt& at, int k0) {
     if (!kSym && g.by_column) {
 #pragma unroll
@@ -287,6 +350,15 @@ __device__ __forceinline__ bool epilogue(const Stage& g, const Job& job, Warp& w
         fetch(next, k0 ^ (blocks & 1));
         fetched = true;
       }
+    }
+    if (EPI == kSquare && parts > 1) {
+      const int slot = ((t - at.z * g.per_matrix) * CG + w.rank) * (4 * CG);
+      if (!add_parts<CG>(sh, g.sums + at.z * g.sums_each + int64_t(slot) * 1024 + mine, w.tmem, w.acc, w.acc_phase, parts, k0,
+                         blocks, lane))
+        return false;
+      w.acc += parts - 1;  // the accumulators of the last part
+      w.acc_phase ^= (w.acc >> 1) & 1;
+      w.acc &= 1;
     }
     if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&sh.acc_full[w.acc]), w.acc_phase, &sh.stop))) return false;
     tc_fence_after();
@@ -383,15 +455,7 @@ __device__ __forceinline__ bool epilogue(const Stage& g, const Job& job, Warp& w
       if (lane == 0) mbar_arrive(smem_u32(&sh.blk_ready[b]));
     }
     w.n += blocks;
-    tc_fence_before();
-    __syncwarp();
-    if (lane == 0) {
-      const uint32_t bar = smem_u32(&sh.acc_empty[w.acc]);
-      if (CG == 2)
-        mbar_arrive_cluster(cluster_map(bar, 0));
-      else
-        mbar_arrive(bar);
-    }
+    release_accumulator<CG>(sh, w.acc, lane);
     if (++w.acc == 2) w.acc = 0, w.acc_phase ^= 1;
   }
   return true;
@@ -593,8 +657,18 @@ __global__ void __launch_bounds__(kGemmThreads, 1) newton_schulz_kernel(const __
           ok = mbar_wait(smem_u32(&sh.acc_empty[acc]), acc_phase ^ 1, &sh.stop);
           if (!ok) break;
           tc_fence_after();
-          const uint32_t d = tmem + acc * kTile;
+          uint32_t d = tmem + acc * kTile;
+          int in_part = 0;
           for (int kb = 0; kb < kblocks; ++kb) {
+            if (in_part == g.part) {  // the next part, into the other accumulators
+              mma_commit<CG>(smem_u32(&sh.acc_full[acc]));
+              if (++acc == 2) acc = 0, acc_phase ^= 1;
+              ok = mbar_wait(smem_u32(&sh.acc_empty[acc]), acc_phase ^ 1, &sh.stop);
+              if (!ok) break;
+              tc_fence_after();
+              d = tmem + acc * kTile;
+              in_part = 0;
+            }
             ok = mbar_wait(smem_u32(&sh.full[slot]), phase, &sh.stop);
             if (!ok) break;
             tc_fence_after();
@@ -602,7 +676,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1) newton_schulz_kernel(const __
             const uint32_t da = smem_desc(a, lead_a), db = smem_desc(b, lead_b);
 #pragma unroll
             for (int k = 0; k < kBK / 16; ++k)
-              mma_f16<CG>(d, da + k * next_a, db + k * next_b, idesc, kb > 0 || k > 0);
+              mma_f16<CG>(d, da + k * next_a, db + k * next_b, idesc, in_part > 0 || k > 0);
+            ++in_part;
             mma_commit<CG>(smem_u32(&sh.empty[slot]));
             if (++slot == kSlots) slot = 0, phase ^= 1;
           }
@@ -814,6 +889,8 @@ int make_stages(NsBatch* shape, const float* coef, int steps, int map0, int coun
     Stage* g = add(kSquare, m, m, n);
     g->mirror = true;
     g->a_mn = g->b_mn = tall;
+    g->sums = reinterpret_cast<float4*>(b.hi[cur ^ 1]);  // (the products that read it are done)
+    g->sums_each = b.plane_x * 2 / int64_t(sizeof(float4));
     g->map_a = g->map_b = uint8_t(map0 + (tall ? kMapXmn : kMapXk) + cur);
     g->map_out = uint8_t(map0 + kMapSqOut);
     g->map_2 = uint8_t(map0 + kMapSqMirror);
@@ -876,6 +953,8 @@ bool cut(Stage* stages, int count, int64_t batch, int cg, int workers, double* w
     g.per_matrix = int(per);
     g.m_fast = g.tiles_m <= g.tiles_n;  // the shorter side first: its operand panels stay in L2
     g.before = before;
+    // (a Gram matrix too large for the free plane is nearly as wide as long: no sum of that one's side is long)
+    g.part = g.sums != nullptr && per * tile * tile * 4 <= g.sums_each * int64_t(sizeof(float4)) ? kPartBlocks : 0x7fffffff;
     before += uint32_t(per) * 2 * cg;   // both store warps of each of its CTAs
     const double tiles = double(per * batch), each = (cg == 1 ? 500.0 : 600.0) * ((g.K + kBK - 1) / kBK);
     const double wait = cg == 1 ? 8e3 : 16e3;

@@ -37,6 +37,9 @@ constexpr int kMatrix = 2 * kPlane;        // high and low plane
 constexpr int kOffS = 0, kOffG = kMatrix, kOffQ = 2 * kMatrix, kBytes = 3 * kMatrix + 2 * kHalfPlane;
 constexpr int kSmemN = kBytes + 1024;
 constexpr int kRing = 6;
+// Pieces of X whose products are accumulated at once; the matrix unit cuts its sums off, which adds up (newton_schulz.cu):
+// 16 x 16777216 was off by 1.5e-2 with all of a CTA's in one sum.
+constexpr int kPartPieces = 256;
 constexpr float kScaleN = 4096.0f;         // planes of G and Q hold 2^12 times theirs, low planes the remainder
 constexpr float kScaleS = 32.0f;           // planes of S: its elements reach the product of all factors
 
@@ -109,6 +112,35 @@ __device__ __forceinline__ void split_mma(uint32_t d, uint32_t ah, uint32_t al, 
     mma_f16<1>(CROSS ? d + 128 : d, a0, b1, idesc, CROSS ? add : true);
     mma_f16<1>(CROSS ? d + 128 : d, a1, b0, idesc, true);
   }
+}
+
+// Adds this warp's accumulators of one more part of a Gram matrix, those of high x high at `tmem` and of the cross terms 128
+// columns further, to the sum of the parts before, 256 columns further; after the last part the sum takes their place.
+// (Not inline: the code of a rare case cost small matrices 2 us.)
+__device__ __noinline__ void add_part(uint32_t tmem, int c0, int np, bool first, bool last) {
+#pragma unroll 1
+  for (; c0 < np; c0 += 64) {
+    uint32_t a[32], b[32];
+    tmem_ld32(tmem + c0, a);
+    tmem_ld32(tmem + 128 + c0, b);
+    tmem_ld_wait();
+#pragma unroll
+    for (int j = 0; j < 32; ++j)
+      a[j] = __float_as_uint(__fmaf_rn(__uint_as_float(b[j]), 1.0f / kScaleLo, __uint_as_float(a[j])));
+    if (!first) {
+      tmem_ld32(tmem + 256 + c0, b);
+      tmem_ld_wait();
+#pragma unroll
+      for (int j = 0; j < 32; ++j) a[j] = __float_as_uint(__uint_as_float(a[j]) + __uint_as_float(b[j]));
+    }
+    tmem_st32(tmem + (last ? 0 : 256) + c0, a);
+    if (last) {
+#pragma unroll
+      for (int j = 0; j < 32; ++j) b[j] = 0;
+      tmem_st32(tmem + 128 + c0, b);
+    }
+  }
+  tmem_st_wait();
 }
 
 __global__ void __launch_bounds__(kThreadsN, 1) narrow_kernel(const __grid_constant__ NarrowArgs p) {
@@ -191,12 +223,15 @@ __global__ void __launch_bounds__(kThreadsN, 1) narrow_kernel(const __grid_const
   // ---- G: high x high into columns 0.., the cross terms (2^11 larger) into columns 128..
   const int gram_slots = nblk == 2 ? 3 : kRing;
   const int gram_pieces = dead ? 0 : pieces;
+  if (warp == 0)
+    for (int i = 0; i < min(gram_pieces, gram_slots); ++i)
+      if (elect_one()) load_piece(i, base + i * piece_bytes, smem_u32(&bars.full[i]));
+  for (int from = 0;; from += kPartPieces) {
+  const int to = min(from + kPartPieces, gram_pieces);
   if (warp == 0) {
     const uint32_t idesc = f16_idesc(128, np, p.tall, p.tall);
     const int ksteps = span / 16;
-    for (int i = 0; i < min(gram_pieces, gram_slots); ++i)
-      if (elect_one()) load_piece(i, base + i * piece_bytes, smem_u32(&bars.full[i]));
-    for (int i = 0; i < gram_pieces; ++i) {
+    for (int i = from; i < to; ++i) {
       const int slot = i % gram_slots;
       wait_full(slot);
       if (!__all_sync(0xffffffffu, ok)) break;
@@ -204,9 +239,9 @@ __global__ void __launch_bounds__(kThreadsN, 1) narrow_kernel(const __grid_const
       if (elect_one()) {
         const uint32_t h = smem_desc(hi, kHalfPlane), l = smem_desc(lo, kHalfPlane);
         if (p.tall)
-          split_mma<true, true, true>(tmem, h, l, h, l, idesc, ksteps, i > 0);
+          split_mma<true, true, true>(tmem, h, l, h, l, idesc, ksteps, i > from);
         else
-          split_mma<false, false, true>(tmem, h, l, h, l, idesc, ksteps, i > 0);
+          split_mma<false, false, true>(tmem, h, l, h, l, idesc, ksteps, i > from);
         mma_commit<1>(smem_u32(&bars.empty[slot]));
       }
       emptied ^= 1u << slot;
@@ -220,6 +255,12 @@ __global__ void __launch_bounds__(kThreadsN, 1) narrow_kernel(const __grid_const
     if (elect_one()) mma_commit<1>(smem_u32(&bars.done[0]));
   }
   wait_done(0);
+  if (gram_pieces > kPartPieces) add_part(lanes, half * 32, np, from == 0, to == gram_pieces);
+  if (to == gram_pieces) break;
+  tc_fence_before();
+  __syncthreads();  // the accumulators are read
+  tc_fence_after();
+  }
   // 2^12 G as fp32, summed over the cluster, as planes into every CTA.
   {
     const uint32_t part = base + kOffS;  // 128 rows of 128 floats
