@@ -35,8 +35,9 @@ constexpr int64_t kApplyChunk = 16384;
 // 4 take 475 us and 8 take 598: fewer CTAs fit an SM.
 constexpr int kGroups = 2;
 constexpr int64_t kMaxPass = 4096;       // matrices of one pass
-// Up to this size one CTA sums, updates and loads a matrix in one launch: 33 us against 37 for all of a
-// 64 x 96 matrix; at 131072 elements (48 of 256 x 512) one CTA for each costs 9 us more than two launches.
+// Up to this size one CTA sums, updates and loads a matrix in one launch.  Two launches / one, us of a whole call: one of
+// 64 x 96 35.7 / 31.8, 128 x 128 53.4 / 49.6, 128 x 256 60.8 / 59.8, 192 x 256 81.2 / 82.7, 256 x 256 85.0 / 89.1;
+// 16 of 128 x 256 62.2 / 61.7, 256 x 256 90.6 / 92.7.
 constexpr int64_t kWholeElems = 32768;
 constexpr int kWholeThreads = 1024;
 constexpr int64_t kSliceBytes = 48 << 20;  // of matrices between the two reads of a slice: they stay in L2
