@@ -99,7 +99,8 @@ def test_every_wait_of_the_kernels_is_this_one():
     narrow = open(os.path.join(CSRC, "newton_schulz_narrow.cu")).read()
     body = narrow[narrow.index("narrow_kernel("):narrow.index("}  // namespace\n")]
     assert body.count("mbar_wait") == body.count("ok &= mbar_wait<true>(") == 3
-    loops = [body[m.start():] for m in re.finditer(r"for \(int i = 0; i < (gram_pieces|todo); \+\+i\)", body)]
+    loops = [body[m.start():] for m in re.finditer(r"for \(int i = (from; i < to|0; i < todo); \+\+i\)", body)]
     assert len(loops) == 2 and len(re.findall(r"< pieces\b", body)) == 0
+    assert "to = min(from + kPartPieces, gram_pieces);" in body and "gram_pieces = dead ? 0 : pieces;" in body
     assert "if (!__all_sync(0xffffffffu, ok)) break;" in loops[0][:300]
     assert "__syncthreads_or(int(stop))) break;" in loops[1][:150]
