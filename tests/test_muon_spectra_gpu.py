@@ -93,3 +93,21 @@ def test_more_steps_do_not_bring_up_noise(shape, merged, kind, steps):
 def test_sixteen_cubic_steps(shape, merged):
     """Steps of small gain: 1.5 each, 657 together."""
     check(spectrum("rank4", *shape, seed=sum(shape)), [(1.5, -0.5, 0.0)] * 16, merged)
+
+
+@pytest.mark.parametrize("shape", [(1, 1), (1, 40), (37, 1), (2, 3), (5, 7), (31, 33), (64, 96), (128, 128), (128, 1000), (1000, 17),
+                                   (16, 9000), (300, 400)], ids=lambda s: "x".join(map(str, s)))
+def test_steps_of_large_gain(shape):
+    """A first step that multiplies by 13, more than the kernel of short sides takes: those run like long ones, and what a
+    single plane's rounding would grow to does not show."""
+    import torch
+    rows = [(13.0, -30.0, 17.5), (1.2, -0.1, 0.0)]
+    gen = torch.Generator(device="cuda").manual_seed(sum(shape))
+    x = torch.randn(3, *shape, generator=gen, device="cuda")
+    from hybridagent_b200 import orthogonalize
+    y = orthogonalize(x, steps=2, coefficients=rows)
+    for k in range(3):
+        want = definition(x[k], rows)
+        # per step: Gram matrix and factor, r / 8 of 30 + 17.5 and 13 at most, on singular values multiplied by 0.5 or more
+        bound = off(want.bfloat16(), want) + 2 * (47.5 + 13) / 0.5 * 0.42 * 2.0 ** -11
+        assert off(y[k], want) <= bound
