@@ -50,10 +50,10 @@
 // to the epilogue warps: products with small K are bound by the epilogue.  Tall matrices (rows > cols) are not
 // transposed: both operand layouts (K contiguous, or M/N contiguous) are read by the MMA as they lie.
 //
-// Measured, from call to result: 4096 x 4096 1.27 ms and 4096 x 12288 2.35 ms, 1.1 PFLOP/s executed (symmetric tiles
-// once), where the chip's power holds large fp16 products at 1.26 to 1.31; two of 17408 x 5120 10.3 ms; 128 of
-// 704 x 2816 3.6 ms, bound by the traffic of X's planes, 0.51 GB each, and by 704 in tiles of 256; 48 of 256 x 512
-// 120 us and 8 of 1024 x 256 103 us, bound by the way from one stage to the next (load, products, epilogue, store,
+// Measured, from call to result: 4096 x 4096 1.25 ms, 1.1 PFLOP/s executed (symmetric tiles once), and 4096 x 12288 2.2 to
+// 2.5 ms, where the chip's power holds fp16 products of 4096 and 8192 in torch at 1.24 and 1.34; two of 17408 x 5120 11.2 ms;
+// 128 of 704 x 2816 3.2 to 3.8 ms, bound by the traffic of X's planes, 0.51 GB each, and by 704 in tiles of 256; 48 of
+// 256 x 512 122 us and 8 of 1024 x 256 105 us, bound by the way from one stage to the next (load, products, epilogue, store,
 // counter: 4 to 8 us).
 #include <cuda.h>
 

@@ -17,8 +17,8 @@
 // steps for itself (which needs no further exchange) and applies S to its columns.  All MMAs have 128 rows;
 // N and K are m rounded up to 16, so small m costs little.
 //
-// Bound by the latency of the products on the m x m side, one after another.  Measured, whole calls: 64 x 96 31 us,
-// 4 of 128 x 2816 85 us, 64 of 32 x 4096 167 us.
+// Bound by the latency of the products on the m x m side, one after another.  Measured, whole calls: 64 x 96 33 us,
+// 4 of 128 x 2816 87 us, 64 of 32 x 4096 171 us.
 #include <cuda.h>
 
 #include <cmath>
