@@ -73,3 +73,25 @@ def test_long_batches_of_several_shapes():
         g, w = (p.grad, p.detach()) if p.shape[0] <= p.shape[1] else (p.grad.mT, p.detach().mT)
         error, rounding = off_and_rounding(-w, g, factor(g))
         assert error <= 1.5 * rounding
+
+
+@pytest.mark.parametrize("shape", [(2, 2000, 40000), (1, 36000, 2100), (3, 300, 33000), (2, 70000, 140)],
+                         ids=lambda s: "x".join(map(str, s)))
+def test_long_batches_alone_and_replayed(shape):
+    """On single CTAs and on pairs, as a graph too, whose second replay finds the first one's sums in the workspace."""
+    import torch
+    from hybridagent_b200 import orthogonalize
+    gen = torch.Generator(device="cuda").manual_seed(sum(shape))
+    x = torch.randn(shape, generator=gen, device="cuda").bfloat16()
+    y = orthogonalize(x)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        z = orthogonalize(x)
+    for _ in range(2):
+        graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(y, z)
+    for k in range(shape[0]):
+        g, w = (x[k].float(), y[k]) if shape[1] <= shape[2] else (x[k].float().mT, y[k].mT)
+        error, rounding = off_and_rounding(w, g, factor(g))
+        assert error <= 1.5 * rounding
