@@ -248,13 +248,13 @@ int ha_adamw_step_delta(const ha_tensor* d_tensors, const ha_chunk* d_chunks, in
 
 /* Newton-Schulz steps X <- a X + (b A + c A A) X with A = X X^T (X taken with rows <= cols; a tall
  * matrix is treated as its transpose), from X = U / max(|U|_F, eps).  Step i uses coef[3i..3i+2] =
- * (a, b, c).  The products run on fp16 operands with fp32 accumulators; X is kept
- * to 22 bits between products until the steps left multiply by no more than 12.  What rounding leaves in directions that U
- * does not have (about 2^-21 of U) grows with every step, 3.44-fold with (3.4445, -4.775, 2.0315): from the ninth
- * or tenth such step on it shows in matrices of low rank, as it does a step or two later in fp32.  Steps that could leave fp16's range are refused: with s the largest
- * singular value a step can meet, |a s + b s^3 + c s^5| up to 4 and |a + b s^2 + c s^4|, |b| s^2 and
- * |c| s^4 up to 60.  eps is between 1e-30 and 1e30; elements of U far
- * below 2^-36 eps vanish. */
+ * (a, b, c).  The products run on fp16 operands with fp32 accumulators; X is kept to 22 bits between
+ * products until the steps left multiply by no more than 12.  What rounding leaves in directions that U does
+ * not have (about 2^-21 of U) grows with every step, 3.44-fold with (3.4445, -4.775, 2.0315): from the ninth or
+ * tenth such step on it shows in matrices of low rank, as it does a step or two later in fp32.  Steps that
+ * could leave fp16's range are refused: with s the largest singular value a step can meet, |a s + b s^3 +
+ * c s^5| up to 4 and |a + b s^2 + c s^4|, |b| s^2 and |c| s^4 up to 60.  eps is between 1e-30 and 1e30;
+ * elements of U far below 2^-36 eps vanish. */
 #define HA_NS_MAX_STEPS 16
 typedef struct ha_ns_params {
   int32_t steps;  /* 1 .. HA_NS_MAX_STEPS */
